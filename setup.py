@@ -34,6 +34,10 @@ setup(
             name="dtensor_muon_b200._C",
             sources=sources,
             extra_compile_args={"cxx": ["-O3", "-std=c++17"], "nvcc": NVCC_FLAGS},
+            # The shared C++ runtime that torch uses. A compiler that finds the static one first would
+            # put a second copy in here, whose streams fault on printing a number: an error message
+            # with one in it would end the process.
+            extra_link_args=["-l:libstdc++.so.6"],
         )
     ],
     cmdclass={"build_ext": BuildExtension.with_options(use_ninja=True)},
