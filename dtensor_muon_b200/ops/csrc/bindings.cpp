@@ -3,7 +3,11 @@
 #include <cuda_runtime.h>
 #include <torch/extension.h>
 
+#include <c10/cuda/CUDAGraphsC10Utils.h>
+
 #include <mutex>
+
+#include "train_ops.h"
 
 namespace dmb {
 
@@ -101,6 +105,8 @@ int* device_error_word(int dev) {
   std::lock_guard<std::mutex> lock(mu);
   if (!words[dev]) {
     c10::cuda::CUDAGuard g(dev);
+    // the first call may come while a graph is captured: the word outlives it
+    c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
     int* p = nullptr;
     C10_CUDA_CHECK(cudaMalloc(&p, sizeof(int)));
     C10_CUDA_CHECK(cudaMemset(p, 0, sizeof(int)));
@@ -160,5 +166,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("swiglu_bwd", &dmb::swiglu_bwd);
   m.def("cross_entropy_fwd", &dmb::cross_entropy_fwd);
   m.def("cross_entropy_bwd", &dmb::cross_entropy_bwd);
+  m.def("launches_counted", &dmb::launches_counted);
   m.def("take_device_error", &dmb::take_device_error);
 }

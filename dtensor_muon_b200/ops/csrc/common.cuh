@@ -19,6 +19,7 @@ enum ErrCode : int {
   kOk = 0,
   kErrGemmPipelineTimeout = 1,
   kErrPeerTimeout = 2,
+  kErrBadIndex = 3,  // a target or position outside its table, in a row that counts
 };
 
 // A wait that makes no progress for this long is treated as a failure: the

@@ -1,0 +1,656 @@
+// Log-probabilities of target tokens and the losses built on them.
+//
+//   logp_t = x_y - log sum_j exp(x_j)                     token_logprobs
+//   policy:      r = exp(logp - old),  d = ref - logp
+//                L = 1/N sum_t m_t (-min(r A, clip(r, 1 - lo, 1 + hi) A) + beta (e^d - 1 - d))
+//   preference:  s_i = sum_t m_t (logp - ref),  h = beta (s_chosen - s_rejected)
+//                L = mean over pairs of -((1 - e) log sigmoid(h) + e log sigmoid(-h))
+//   gradient of any of them: dx_j = c_t ([j == y] - softmax(x)_j), c_t = dL / dlogp_t
+//
+// One pass over the logits forward (running maximum m and sum s per thread, joined over the
+// row), one read and one write backward. The statistics kept between the two are (m, s) and not
+// the log-sum-exp: exp(x - m) / s has no large terms that cancel, so its relative error does not
+// grow with the size of the logits. What follows from a row's logp (ratio, KL estimate, their
+// derivatives) is computed in 64 bits by the one thread that joins the row, from x_y - m and s:
+// differences of log-probabilities nearly cancel, and rounding them first would be what is lost.
+// Rows that do not count are not read.
+#include <ATen/ATen.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <cooperative_groups.h>
+
+#include "train_ops.h"
+#include "vec.cuh"
+
+namespace dmb {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2eRest = (float)(1.4426950408889634 - (double)kLog2e);
+constexpr int kUnroll = 4;         // 8-element vectors in flight per thread
+constexpr int kRowThreads = 512;   // threads of a CTA that shares a row
+constexpr int kWarpRows = 4;       // rows of a CTA whose warps have one each
+
+enum Mode { kLogprob, kPolicy, kPreference };
+
+struct RowArgs {
+  const void* logits;
+  long long stride_b, stride_s;  // elements
+  int seq;                       // rows per stride_b
+  int rows, vocab;
+  const int64_t* targets;
+  const bool* mask;  // null: every row counts
+  float* logp;
+  float2* stats;  // (m, s) of each row
+  int* error;
+  // policy and preference
+  const float *old_logp, *advantages, *ref_logp;
+  float clip_low, clip_high, kl_coef;
+  float *row_loss, *row_kl, *coef;
+  bool* row_clipped;
+  double* row_diff;
+};
+
+// Only of values that are at most 0, as they are taken against a maximum. Results below 2^-126 become 0: next to the
+// maximum's own 1 they add nothing to a sum, and a probability that small is below what a gradient can hold.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// (a - m) * log2 e of two values at once. EXACT adds what the constant loses in 32 bits: 1.3e-8 of the product, always to
+// the same side, which a sum of a thousand log-probabilities (a sequence's log ratio) would show.
+template <bool EXACT>
+__device__ __forceinline__ void scaled2(float& a, float& b, float neg_m) {
+  if constexpr (EXACT) {
+    asm("{\n\t.reg .b64 v, m, c, d, t;\n\t"
+        "mov.b64 v, {%0, %1};\n\t"
+        "mov.b64 m, {%2, %2};\n\t"
+        "mov.b64 c, {%3, %3};\n\t"
+        "mov.b64 d, {%4, %4};\n\t"
+        "add.rn.f32x2 v, v, m;\n\t"
+        "mul.rn.f32x2 t, v, d;\n\t"
+        "fma.rn.f32x2 v, v, c, t;\n\t"
+        "mov.b64 {%0, %1}, v;\n\t}"
+        : "+f"(a), "+f"(b)
+        : "f"(neg_m), "f"(kLog2e), "f"(kLog2eRest));
+  } else {
+    asm("{\n\t.reg .b64 v, m, c;\n\t"
+        "mov.b64 v, {%0, %1};\n\t"
+        "mov.b64 m, {%2, %2};\n\t"
+        "mov.b64 c, {%3, %3};\n\t"
+        "add.rn.f32x2 v, v, m;\n\t"
+        "mul.rn.f32x2 v, v, c;\n\t"
+        "mov.b64 {%0, %1}, v;\n\t}"
+        : "+f"(a), "+f"(b)
+        : "f"(neg_m), "f"(kLog2e));
+  }
+}
+
+// What exponents are taken against: a row (or part) of nothing but -inf has no finite maximum.
+__device__ __forceinline__ float anchor(float m) { return m == -INFINITY ? 0.f : m; }
+
+// Joins two parts. expf and not ex2: what a sum is multiplied with again and again should not lean to one side.
+__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
+  const float mx = fmaxf(m, m2), a = anchor(mx);
+  s = (m == mx ? s : s * expf(m - a)) + (m2 == mx ? s2 : s2 * expf(m2 - a));
+  m = mx;
+}
+
+// A warp's parts joined: the maximum first, so that each sum is scaled once. Every lane gets the result.
+__device__ __forceinline__ void warp_join(float& m, float& s) {
+  float mx = m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, o));
+  s *= expf(m - anchor(mx));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+  m = mx;
+}
+
+template <typename T>
+__device__ __forceinline__ const T* row_of(const void* logits, long long stride_b, long long stride_s, int seq, int row) {
+  return static_cast<const T*>(logits) + (long long)(row / seq) * stride_b + (long long)(row % seq) * stride_s;
+}
+
+// Elements in front of a row's first 16-byte boundary.
+template <typename T>
+__device__ __forceinline__ int head_of(const T* p, int n) {
+  const int h = (int)(((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T));
+  return min(h, n);
+}
+
+template <typename T>
+__device__ __forceinline__ Raw8<T> raw_neg_inf() {
+  Raw8<T> r;
+  const uint32_t w = sizeof(T) == 4 ? 0xFF800000u : std::is_same<T, __nv_bfloat16>::value ? 0xFF80FF80u : 0xFC00FC00u;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.w[i] = make_uint4(w, w, w, w);
+  return r;
+}
+
+// Maximum and sum of exponentials of one thread's share of p[0, n): threads `tid` of `nt`, and
+// the vectors [v0, v1) of the row's; the ends that no vector covers go to `ends`.
+template <typename T>
+__device__ __forceinline__ void scan_row(const T* p, int n, int head, int v0, int v1, int tid, int nt, bool ends,
+                                         float& m, float& s) {
+  m = -INFINITY;
+  s = 0.f;
+  const T* body = p + head;
+  for (int base = v0 + tid; base < v1; base += nt * kUnroll) {
+    Raw8<T> raw[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int v = base + u * nt;
+      raw[u] = v < v1 ? load_raw8<T>(body + (long long)v * 8) : raw_neg_inf<T>();
+    }
+    float f[kUnroll][8], mx = m;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      unpack8<T>(raw[u], f[u]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) mx = fmaxf(mx, f[u][k]);
+    }
+    const float a = anchor(mx);
+    float part[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+#pragma unroll
+      for (int k = 0; k < 8; k += 2) scaled2<true>(f[u][k], f[u][k + 1], -a);
+      float e0 = ex2(f[u][0]), e1 = ex2(f[u][1]);
+#pragma unroll
+      for (int k = 2; k < 8; k += 2) {
+        e0 += ex2(f[u][k]);
+        e1 += ex2(f[u][k + 1]);
+      }
+      part[u] = e0 + e1;
+    }
+    s = s * expf(m - a) + ((part[0] + part[1]) + (part[2] + part[3]));
+    m = mx;
+  }
+  if (ends) {
+    const int tail = head + (n - head) / 8 * 8;
+    for (int j = tid; j < head + (n - tail); j += nt) join(m, s, to_float(p[j < head ? j : tail + j - head]), 1.f);
+  }
+}
+
+// What one thread does once a row's maximum and sum are known.
+template <Mode MODE>
+__device__ __forceinline__ void finish_row(const RowArgs& a, int row, float xy, float m, float s) {
+  // ex2.approx comes out low on average: by 2e-8 of its value above 1/2 and by 5e-8 in every octave below (measured). One
+  // token does not show it, but a sequence's sum of a thousand log-probabilities does. A thread takes its exponentials
+  // against its own maximum, so that most of its sum is near 1: 2e-8 is what a row's sum is low by. The maximum is exact.
+  constexpr double kLow = 2.0e-8;
+  const double lp = ((double)xy - (double)anchor(m)) - log((double)s + kLow * ((double)s - 1.0));
+  a.logp[row] = (float)lp;
+  a.stats[row] = make_float2(anchor(m), s);
+  if constexpr (MODE == kPolicy) {
+    const double adv = a.advantages[row], ratio = exp(lp - (double)a.old_logp[row]);
+    const double held_ratio = ratio < 1.0 - a.clip_low ? 1.0 - a.clip_low : ratio > 1.0 + a.clip_high ? 1.0 + a.clip_high : ratio;
+    const double open = ratio * adv, held = held_ratio * adv;
+    const bool clipped = open > held;
+    double loss = -(clipped ? held : open), coef = clipped ? 0.0 : -open, kl = 0.0;
+    if (a.ref_logp) {
+      const double d = (double)a.ref_logp[row] - lp, e = expm1(d);
+      kl = e - d;
+      if (a.kl_coef != 0.f) {
+        loss += (double)a.kl_coef * kl;
+        coef -= (double)a.kl_coef * e;
+      }
+    }
+    a.row_loss[row] = (float)loss;
+    a.row_kl[row] = (float)kl;
+    a.row_clipped[row] = clipped;
+    a.coef[row] = (float)coef;
+  }
+  if constexpr (MODE == kPreference) a.row_diff[row] = lp - (double)a.ref_logp[row];
+}
+
+template <Mode MODE>
+__device__ __forceinline__ void skip_row(const RowArgs& a, int row) {
+  a.logp[row] = 0.f;
+  a.stats[row] = make_float2(0.f, 1.f);
+  if constexpr (MODE == kPolicy) {
+    a.row_loss[row] = 0.f;
+    a.row_kl[row] = 0.f;
+    a.row_clipped[row] = false;
+    a.coef[row] = 0.f;
+  }
+  if constexpr (MODE == kPreference) a.row_diff[row] = 0.0;
+}
+
+template <typename T>
+__device__ __forceinline__ float target_logit(const RowArgs& a, const T* p, int row) {
+  const int64_t y = a.targets[row];
+  if (y < 0 || y >= a.vocab) {
+    atomicExch(a.error, (int)kErrBadIndex);
+    return NAN;
+  }
+  return to_float(p[y]);
+}
+
+// One warp per row, for short rows.
+template <typename T, Mode MODE>
+__global__ void __launch_bounds__(32 * kWarpRows) warp_row_kernel(const RowArgs a) {
+  const int row = blockIdx.x * kWarpRows + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= a.rows) return;
+  if (a.mask && !a.mask[row]) {
+    if (lane == 0) skip_row<MODE>(a, row);
+    return;
+  }
+  const T* p = row_of<T>(a.logits, a.stride_b, a.stride_s, a.seq, row);
+  const int head = head_of(p, a.vocab);
+  const float xy = lane == 0 ? target_logit(a, p, row) : 0.f;
+  float m, s;
+  scan_row<T>(p, a.vocab, head, 0, (a.vocab - head) / 8, lane, 32, true, m, s);
+  warp_join(m, s);
+  if (lane == 0) finish_row<MODE>(a, row, xy, m, s);
+}
+
+// One cluster of CTAs per row (often a cluster of one). With fewer rows than the GPU has room for, a row is
+// split over the cluster's CTAs, which hand their maximum and sum to the first one's shared memory.
+template <typename T, Mode MODE>
+__global__ void __launch_bounds__(kRowThreads) row_kernel(const RowArgs a) {
+  __shared__ float2 warps[kRowThreads / 32];
+  __shared__ float2 parts[8];  // of the cluster's CTAs, in the first one
+  cg::cluster_group cluster = cg::this_cluster();
+  const int split = cluster.num_blocks(), rank = cluster.block_rank();
+  const int row = blockIdx.x / split;
+  if (a.mask && !a.mask[row]) {  // the whole cluster leaves
+    if (rank == 0 && threadIdx.x == 0) skip_row<MODE>(a, row);
+    return;
+  }
+  if (split > 1) cluster.barrier_arrive();  // waited for below: all have begun before one writes to another
+  const T* p = row_of<T>(a.logits, a.stride_b, a.stride_s, a.seq, row);
+  const int head = head_of(p, a.vocab), vecs = (a.vocab - head) / 8;
+  const float xy = rank == 0 && threadIdx.x == 0 ? target_logit(a, p, row) : 0.f;
+  float m, s;
+  scan_row<T>(p, a.vocab, head, (int)((long long)vecs * rank / split), (int)((long long)vecs * (rank + 1) / split),
+              threadIdx.x, kRowThreads, rank == 0, m, s);
+  warp_join(m, s);
+  if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = make_float2(m, s);
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const float2 w = threadIdx.x < kRowThreads / 32 ? warps[threadIdx.x] : make_float2(-INFINITY, 0.f);
+    m = w.x;
+    s = w.y;
+    warp_join(m, s);
+  }
+  if (split > 1) {
+    cluster.barrier_wait();
+    if (threadIdx.x == 0) *cluster.map_shared_rank(&parts[rank], 0) = make_float2(m, s);
+    cluster.sync();
+    if (rank == 0 && threadIdx.x == 0)
+      for (int i = 1; i < split; ++i) join(m, s, parts[i].x, parts[i].y);
+  }
+  if (rank == 0 && threadIdx.x == 0) finish_row<MODE>(a, row, xy, m, s);
+}
+
+struct GradArgs {
+  const void* logits;
+  long long stride_b, stride_s;
+  int seq, rows, vocab, chunks;
+  int rows_per_coef;
+  const int64_t* targets;
+  const bool* mask;
+  const float* coef;
+  const float* scale;  // null: 1
+  const float2* stats;
+  void* grad;  // contiguous
+};
+
+constexpr int kGradThreads = 256;
+
+// dx_j = c ([j == y] - exp(x_j - m) / s). Each CTA takes one of a row's `chunks`. Rows with c = 0 are not read.
+template <typename T>
+__global__ void __launch_bounds__(kGradThreads) logprob_grad_kernel(const GradArgs a) {
+  const int row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
+  const int n = a.vocab;
+  T* g = static_cast<T*>(a.grad) + (long long)row * n;
+  float c = a.mask && !a.mask[row] ? 0.f : a.coef[row / a.rows_per_coef];
+  if (c != 0.f && a.scale) c *= *a.scale;
+  const int g_head = head_of(g, n), vecs = (n - g_head) / 8;
+  const int v0 = (int)((long long)vecs * chunk / a.chunks), v1 = (int)((long long)vecs * (chunk + 1) / a.chunks);
+  const int tail = g_head + vecs * 8;
+  if (c == 0.f) {
+    const float zero[8] = {};
+    for (int v = v0 + threadIdx.x; v < v1; v += kGradThreads) store8t<T>(g + g_head + (long long)v * 8, zero);
+    if (chunk == 0)
+      for (int j = threadIdx.x; j < g_head + (n - tail); j += kGradThreads)
+        g[j < g_head ? j : tail + j - g_head] = from_float<T>(0.f);
+    return;
+  }
+  const T* p = row_of<T>(a.logits, a.stride_b, a.stride_s, a.seq, row);
+  const float2 st = a.stats[row];
+  const float m = st.x, neg = -c / st.y;
+  const int y = (int)a.targets[row];
+  auto one = [&](int j) {
+    const float e = ex2((to_float(p[j]) - m) * kLog2e);
+    g[j] = from_float<T>(fmaf(neg, e, j == y ? c : 0.f));
+  };
+  if (((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0) {
+    const T *src = p + g_head;
+    T* dst = g + g_head;
+    const int yv = y >= g_head ? (y - g_head) / 8 : -1, yk = (y - g_head) & 7;
+    for (int base = v0 + threadIdx.x; base < v1; base += kGradThreads * kUnroll) {
+      Raw8<T> raw[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int v = base + u * kGradThreads;
+        if (v < v1) raw[u] = load_raw8<T>(src + (long long)v * 8);
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int v = base + u * kGradThreads;
+        if (v >= v1) break;
+        float f[8];
+        unpack8<T>(raw[u], f);
+#pragma unroll
+        for (int k = 0; k < 8; k += 2) scaled2<false>(f[k], f[k + 1], -m);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] = neg * ex2(f[k]);
+        if (v == yv) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) f[k] += k == yk ? c : 0.f;
+        }
+        store8t<T>(dst + (long long)v * 8, f);
+      }
+    }
+  } else {  // the gradient's rows lie on other boundaries than the logits'
+    for (int j = g_head + v0 * 8 + threadIdx.x; j < g_head + v1 * 8; j += kGradThreads) one(j);
+  }
+  if (chunk == 0)
+    for (int j = threadIdx.x; j < g_head + (n - tail); j += kGradThreads) one(j < g_head ? j : tail + j - g_head);
+}
+
+constexpr int kReduceThreads = 1024;
+
+// Sum over the CTA, the same order in every run; every thread gets it.
+__device__ __forceinline__ double block_sum(double v, double* smem) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = smem[threadIdx.x & 31];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  return v;
+}
+
+// Means over the rows that count, and the rows' coefficients divided by their number. One CTA: the rows' values are
+// a vocabulary's size less than what the row kernel read.
+__global__ void __launch_bounds__(kReduceThreads) policy_reduce_kernel(const RowArgs a, float* loss, float* kl, float* clipped) {
+  __shared__ double smem[32];
+  double l = 0, d = 0, c = 0, n = 0;
+  for (int i = threadIdx.x; i < a.rows; i += kReduceThreads) {
+    l += a.row_loss[i];
+    d += a.row_kl[i];
+    c += a.row_clipped[i] ? 1 : 0;
+    n += !a.mask || a.mask[i] ? 1 : 0;
+  }
+  l = block_sum(l, smem);
+  d = block_sum(d, smem);
+  c = block_sum(c, smem);
+  n = block_sum(n, smem);
+  const double inv = n > 0 ? 1.0 / n : 0.0;
+  if (threadIdx.x == 0) {
+    *loss = (float)(l * inv);
+    *kl = (float)(d * inv);
+    *clipped = (float)(c * inv);
+  }
+  for (int i = threadIdx.x; i < a.rows; i += kReduceThreads) a.coef[i] = (float)(a.coef[i] * inv);
+}
+
+// A warp sums each sequence, then a thread takes each pair. coef[i] is the derivative by each of sequence i's logp.
+__global__ void __launch_bounds__(kReduceThreads) preference_reduce_kernel(const double* diff, int pairs, int seq, float beta,
+                                                                          float smoothing, double* sums, float* loss,
+                                                                          float* rewards, float* coef) {
+  __shared__ double smem[32];
+  const int lane = threadIdx.x & 31;
+  for (int i = threadIdx.x >> 5; i < 2 * pairs; i += kReduceThreads / 32) {
+    double v = 0;
+    for (int t = lane; t < seq; t += 32) v += diff[(long long)i * seq + t];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+    if (lane == 0) {
+      sums[i] = v;
+      rewards[i] = (float)(beta * v);
+    }
+  }
+  __syncthreads();
+  double l = 0;
+  for (int i = threadIdx.x; i < pairs; i += kReduceThreads) {
+    const double h = (double)beta * (sums[i] - sums[pairs + i]);
+    const double tail = log1p(exp(-fabs(h)));  // log sigmoid(h) = min(h, 0) - tail
+    const double up = fmin(h, 0.0) - tail, down = fmin(-h, 0.0) - tail;
+    l -= (1.0 - smoothing) * up + smoothing * down;
+    const double sig = h >= 0 ? 1.0 / (1.0 + exp(-h)) : exp(h) / (1.0 + exp(h));
+    const double dh = (double)smoothing * sig - (1.0 - smoothing) * (1.0 - sig);
+    coef[i] = (float)(beta * dh / pairs);
+    coef[pairs + i] = (float)(-beta * dh / pairs);
+  }
+  l = block_sum(l, smem);
+  if (threadIdx.x == 0) *loss = (float)(l / pairs);
+}
+
+// ------------------------------------------------------------------ host
+
+struct Rows {
+  at::Tensor logits;  // [.., V], last stride 1; two or three dims
+  long long stride_b, stride_s;
+  int seq, rows, vocab;
+};
+
+Rows rows_of(const at::Tensor& logits, const at::Tensor& targets, const OptTensor& mask) {
+  TORCH_CHECK_VALUE(logits.is_cuda(), "logits: CUDA tensor expected");
+  const auto t = logits.scalar_type();
+  TORCH_CHECK_VALUE(t == at::kFloat || t == at::kBFloat16 || t == at::kHalf, "logits: float32, bfloat16 or float16 expected, got ", t);
+  TORCH_CHECK_VALUE(logits.dim() >= 2 && logits.size(-1) > 0, "logits: [..., vocab] with a vocabulary expected");
+  TORCH_CHECK_VALUE(targets.scalar_type() == at::kLong && targets.device() == logits.device() &&
+                        targets.sizes() == logits.sizes().slice(0, logits.dim() - 1),
+                    "targets: int64 tensor of the logits' leading shape on their device expected");
+  if (mask.has_value())
+    TORCH_CHECK_VALUE(mask->scalar_type() == at::kBool && mask->device() == logits.device() && mask->sizes() == targets.sizes(),
+                      "mask: bool tensor of the targets' shape on their device expected");
+  const long long n = targets.numel(), v = logits.size(-1);
+  TORCH_CHECK_VALUE(n < (1ll << 31) / 32 && v < (1ll << 30), "at most 2^26 rows of 2^30 logits expected, got ", n, " of ", v);
+  Rows r;
+  r.logits = logits;
+  if (logits.dim() > 3) r.logits = logits.reshape({-1, v});
+  if (r.logits.stride(-1) != 1 && v > 1) r.logits = r.logits.contiguous();
+  const bool three = r.logits.dim() == 3;
+  r.stride_b = three ? r.logits.stride(0) : 0;
+  r.stride_s = r.logits.stride(-2);
+  r.seq = (int)std::max<int64_t>(1, r.logits.size(-2));
+  r.rows = (int)n;
+  r.vocab = (int)v;
+  return r;
+}
+
+at::Tensor row_values(const at::Tensor& v, const at::Tensor& targets, const char* name) {
+  TORCH_CHECK_VALUE(v.scalar_type() == at::kFloat && v.device() == targets.device() && v.sizes() == targets.sizes(), name,
+                    ": float32 tensor of the targets' shape on their device expected");
+  return v.contiguous();
+}
+
+// Rows up to this length go to a warp each: 8 vectors per lane. (A CTA's 512 threads would have less than one each.)
+constexpr int kWarpRowMax = 2048;
+
+template <Mode MODE>
+void launch_rows(const Rows& r, RowArgs a, cudaStream_t stream) {
+  a.logits = r.logits.const_data_ptr();
+  a.stride_b = r.stride_b;
+  a.stride_s = r.stride_s;
+  a.seq = r.seq;
+  a.rows = r.rows;
+  a.vocab = r.vocab;
+  a.error = device_error_word(r.logits.device().index());
+  if (r.rows == 0) return;
+  with_element(r.logits.scalar_type(), [&](auto* tag) {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    if (r.vocab <= kWarpRowMax) {
+      warp_row_kernel<T, MODE><<<(r.rows + kWarpRows - 1) / kWarpRows, 32 * kWarpRows, 0, stream>>>(a);
+      C10_CUDA_KERNEL_LAUNCH_CHECK();
+    } else {
+      // Few rows: split each until every SM has two CTAs or a part is down to one round of its CTA's loads.
+      const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+      int split = 1;
+      while (split < 8 && (long long)r.rows * split < 2 * sms && r.vocab / split > 2 * kRowThreads * 8 * kUnroll) split *= 2;
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3((unsigned)r.rows * split);
+      cfg.blockDim = dim3(kRowThreads);
+      cfg.stream = stream;
+      cudaLaunchAttribute attr;
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim = {(unsigned)split, 1, 1};
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+      C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, row_kernel<T, MODE>, a));
+    }
+  });
+  count_launches(1);
+}
+
+}  // namespace
+
+std::tuple<at::Tensor, at::Tensor> token_logprobs_fwd(const at::Tensor& logits, const at::Tensor& targets,
+                                                      const OptTensor& mask) {
+  const Rows r = rows_of(logits, targets, mask);
+  const c10::cuda::CUDAGuard guard(logits.device());
+  const auto f32 = logits.options().dtype(at::kFloat);
+  auto logp = at::empty(targets.sizes(), f32), stats = at::empty({r.rows, 2}, f32);
+  const auto t = targets.contiguous();
+  const auto m = mask.has_value() ? mask->contiguous() : at::Tensor();
+  RowArgs a = {};
+  a.targets = t.const_data_ptr<int64_t>();
+  a.mask = m.defined() ? m.const_data_ptr<bool>() : nullptr;
+  a.logp = logp.mutable_data_ptr<float>();
+  a.stats = reinterpret_cast<float2*>(stats.mutable_data_ptr<float>());
+  launch_rows<kLogprob>(r, a, at::cuda::getCurrentCUDAStream());
+  return {logp, stats};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> policy_loss_fwd(
+    const at::Tensor& logits, const at::Tensor& targets, const at::Tensor& old_logp, const at::Tensor& advantages,
+    const OptTensor& ref_logp, const OptTensor& mask, double clip_low, double clip_high, double kl_coef) {
+  const Rows r = rows_of(logits, targets, mask);
+  TORCH_CHECK_VALUE(clip_low >= 0 && clip_low <= 1 && clip_high >= 0, "clip_low in [0, 1] and clip_high >= 0 expected, got ",
+                    clip_low, " and ", clip_high);
+  TORCH_CHECK_VALUE(kl_coef == 0 || ref_logp.has_value(), "kl_coef needs ref_logp");
+  const c10::cuda::CUDAGuard guard(logits.device());
+  const auto f32 = logits.options().dtype(at::kFloat);
+  const auto t = targets.contiguous(), old = row_values(old_logp, targets, "old_logp"),
+             adv = row_values(advantages, targets, "advantages");
+  const auto ref = ref_logp.has_value() ? row_values(*ref_logp, targets, "ref_logp") : at::Tensor();
+  const auto m = mask.has_value() ? mask->contiguous() : at::Tensor();
+  auto loss = at::empty({}, f32), kl = at::empty({}, f32), clipped = at::empty({}, f32);
+  auto logp = at::empty(targets.sizes(), f32), coef = at::empty(targets.sizes(), f32), stats = at::empty({r.rows, 2}, f32);
+  auto row = at::empty({2, r.rows}, f32), row_clipped = at::empty({r.rows}, f32.dtype(at::kBool));
+  RowArgs a = {};
+  a.targets = t.const_data_ptr<int64_t>();
+  a.mask = m.defined() ? m.const_data_ptr<bool>() : nullptr;
+  a.logp = logp.mutable_data_ptr<float>();
+  a.stats = reinterpret_cast<float2*>(stats.mutable_data_ptr<float>());
+  a.old_logp = old.const_data_ptr<float>();
+  a.advantages = adv.const_data_ptr<float>();
+  a.ref_logp = ref.defined() ? ref.const_data_ptr<float>() : nullptr;
+  a.clip_low = (float)clip_low;
+  a.clip_high = (float)clip_high;
+  a.kl_coef = (float)kl_coef;
+  a.row_loss = row.mutable_data_ptr<float>();
+  a.row_kl = a.row_loss + r.rows;
+  a.row_clipped = row_clipped.mutable_data_ptr<bool>();
+  a.coef = coef.mutable_data_ptr<float>();
+  const auto stream = at::cuda::getCurrentCUDAStream();
+  launch_rows<kPolicy>(r, a, stream);
+  a.rows = r.rows;
+  policy_reduce_kernel<<<1, kReduceThreads, 0, stream>>>(a, loss.mutable_data_ptr<float>(), kl.mutable_data_ptr<float>(),
+                                                        clipped.mutable_data_ptr<float>());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  count_launches(1);
+  return {loss, logp, kl, clipped, stats, coef};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> preference_loss_fwd(
+    const at::Tensor& logits, const at::Tensor& targets, const at::Tensor& ref_logp, const OptTensor& mask, double beta,
+    double label_smoothing) {
+  const Rows r = rows_of(logits, targets, mask);
+  TORCH_CHECK_VALUE(targets.dim() == 2 && targets.size(0) > 0 && targets.size(0) % 2 == 0,
+                    "targets: [2 * pairs, seq] expected, the chosen sequences in front of the rejected ones");
+  TORCH_CHECK_VALUE(beta > 0 && label_smoothing >= 0 && label_smoothing < 0.5,
+                    "beta > 0 and label_smoothing in [0, 0.5) expected, got ", beta, " and ", label_smoothing);
+  const c10::cuda::CUDAGuard guard(logits.device());
+  const auto f32 = logits.options().dtype(at::kFloat), f64 = logits.options().dtype(at::kDouble);
+  const auto t = targets.contiguous(), ref = row_values(ref_logp, targets, "ref_logp");
+  const auto m = mask.has_value() ? mask->contiguous() : at::Tensor();
+  const int seqs = (int)targets.size(0), seq = (int)targets.size(1);
+  auto loss = at::empty({}, f32), rewards = at::empty({seqs}, f32), coef = at::empty({seqs}, f32);
+  auto logp = at::empty(targets.sizes(), f32), stats = at::empty({r.rows, 2}, f32);
+  auto wide = at::empty({r.rows + seqs}, f64);
+  RowArgs a = {};
+  a.targets = t.const_data_ptr<int64_t>();
+  a.mask = m.defined() ? m.const_data_ptr<bool>() : nullptr;
+  a.logp = logp.mutable_data_ptr<float>();
+  a.stats = reinterpret_cast<float2*>(stats.mutable_data_ptr<float>());
+  a.ref_logp = ref.const_data_ptr<float>();
+  a.row_diff = wide.mutable_data_ptr<double>();
+  const auto stream = at::cuda::getCurrentCUDAStream();
+  launch_rows<kPreference>(r, a, stream);
+  preference_reduce_kernel<<<1, kReduceThreads, 0, stream>>>(a.row_diff, seqs / 2, seq, (float)beta, (float)label_smoothing,
+                                                            a.row_diff + r.rows, loss.mutable_data_ptr<float>(),
+                                                            rewards.mutable_data_ptr<float>(), coef.mutable_data_ptr<float>());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  count_launches(1);
+  return {loss, logp, rewards, stats, coef};
+}
+
+at::Tensor token_logprobs_bwd(const at::Tensor& coef, const OptTensor& scale, const at::Tensor& logits,
+                              const at::Tensor& targets, const at::Tensor& stats, const OptTensor& mask) {
+  const Rows r = rows_of(logits, targets, mask);
+  TORCH_CHECK_VALUE(coef.scalar_type() == at::kFloat && coef.device() == logits.device() &&
+                        (coef.sizes() == targets.sizes() || (targets.dim() == 2 && coef.dim() == 1 && coef.size(0) == targets.size(0))),
+                    "coef: float32 per target or per sequence expected");
+  TORCH_CHECK_VALUE(stats.scalar_type() == at::kFloat && stats.device() == logits.device() && stats.is_contiguous() &&
+                        stats.dim() == 2 && stats.size(0) == r.rows && stats.size(1) == 2,
+                    "stats: contiguous float32 [rows, 2] expected");
+  if (scale.has_value())
+    TORCH_CHECK_VALUE(scale->scalar_type() == at::kFloat && scale->device() == logits.device() && scale->numel() == 1,
+                      "scale: one float32 value expected");
+  const c10::cuda::CUDAGuard guard(logits.device());
+  auto grad = at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
+  if (r.rows == 0) return grad;
+  const auto t = targets.contiguous(), cf = coef.contiguous();
+  const auto m = mask.has_value() ? mask->contiguous() : at::Tensor();
+  GradArgs a = {};
+  a.logits = r.logits.const_data_ptr();
+  a.stride_b = r.stride_b;
+  a.stride_s = r.stride_s;
+  a.seq = r.seq;
+  a.rows = r.rows;
+  a.vocab = r.vocab;
+  a.rows_per_coef = (int)(r.rows / coef.numel());
+  a.targets = t.const_data_ptr<int64_t>();
+  a.mask = m.defined() ? m.const_data_ptr<bool>() : nullptr;
+  a.coef = cf.const_data_ptr<float>();
+  a.scale = scale.has_value() ? scale->const_data_ptr<float>() : nullptr;
+  a.stats = reinterpret_cast<const float2*>(stats.const_data_ptr<float>());
+  a.grad = grad.mutable_data_ptr();
+  // two rounds of a CTA's loads for each chunk
+  const int per = kGradThreads * 8 * kUnroll * 2;
+  a.chunks = std::max(1, (r.vocab + per - 1) / per);
+  TORCH_CHECK_VALUE((long long)a.chunks * r.rows < (1ll << 31), "logits: too many values for one call");
+  with_element(logits.scalar_type(), [&](auto* tag) {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    logprob_grad_kernel<T><<<(unsigned)(a.chunks * r.rows), kGradThreads, 0, at::cuda::getCurrentCUDAStream()>>>(a);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  });
+  count_launches(1);
+  return grad;
+}
+
+}  // namespace dmb
