@@ -18,7 +18,10 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <cooperative_groups.h>
+
+#include <climits>
 
 #include "train_ops.h"
 #include "vec.cuh"
@@ -30,8 +33,7 @@ namespace cg = cooperative_groups;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLog2eRest = (float)(1.4426950408889634 - (double)kLog2e);
-constexpr int kUnroll = 4;         // 8-element vectors in flight per thread
-constexpr int kRowThreads = 512;   // threads of a CTA that shares a row
+constexpr int kUnroll = 4;         // 8-element vectors that a thread takes at once
 constexpr int kWarpRows = 4;       // rows of a CTA whose warps have one each
 
 enum Mode { kLogprob, kPolicy, kPreference };
@@ -49,9 +51,11 @@ struct RowArgs {
   // policy and preference
   const float *old_logp, *advantages, *ref_logp;
   float clip_low, clip_high, kl_coef;
+  const int* count;  // rows that the mask keeps; null: all
   float *row_loss, *row_kl, *coef;
   bool* row_clipped;
   double* row_diff;
+  void* grad;  // contiguous; null: no gradient
 };
 
 // Only of values that are at most 0, as they are taken against a maximum. Results below 2^-126 become 0: next to the
@@ -62,33 +66,9 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// (a - m) * log2 e of two values at once. EXACT adds what the constant loses in 32 bits: 1.3e-8 of the product, always to
-// the same side, which a sum of a thousand log-probabilities (a sequence's log ratio) would show.
-template <bool EXACT>
-__device__ __forceinline__ void scaled2(float& a, float& b, float neg_m) {
-  if constexpr (EXACT) {
-    asm("{\n\t.reg .b64 v, m, c, d, t;\n\t"
-        "mov.b64 v, {%0, %1};\n\t"
-        "mov.b64 m, {%2, %2};\n\t"
-        "mov.b64 c, {%3, %3};\n\t"
-        "mov.b64 d, {%4, %4};\n\t"
-        "add.rn.f32x2 v, v, m;\n\t"
-        "mul.rn.f32x2 t, v, d;\n\t"
-        "fma.rn.f32x2 v, v, c, t;\n\t"
-        "mov.b64 {%0, %1}, v;\n\t}"
-        : "+f"(a), "+f"(b)
-        : "f"(neg_m), "f"(kLog2e), "f"(kLog2eRest));
-  } else {
-    asm("{\n\t.reg .b64 v, m, c;\n\t"
-        "mov.b64 v, {%0, %1};\n\t"
-        "mov.b64 m, {%2, %2};\n\t"
-        "mov.b64 c, {%3, %3};\n\t"
-        "add.rn.f32x2 v, v, m;\n\t"
-        "mul.rn.f32x2 v, v, c;\n\t"
-        "mov.b64 {%0, %1}, v;\n\t}"
-        : "+f"(a), "+f"(b)
-        : "f"(neg_m), "f"(kLog2e));
-  }
+__device__ __forceinline__ F2 ex2(F2 x) {
+  const float2 v = f2_values(x);
+  return f2(ex2(v.x), ex2(v.y));
 }
 
 // What exponents are taken against: a row (or part) of nothing but -inf has no finite maximum.
@@ -114,7 +94,8 @@ __device__ __forceinline__ void warp_join(float& m, float& s) {
 
 template <typename T>
 __device__ __forceinline__ const T* row_of(const void* logits, long long stride_b, long long stride_s, int seq, int row) {
-  return static_cast<const T*>(logits) + (long long)(row / seq) * stride_b + (long long)(row % seq) * stride_s;
+  const unsigned b = (unsigned)row / (unsigned)seq, s = row - b * seq;
+  return static_cast<const T*>(logits) + b * stride_b + s * stride_s;
 }
 
 // Elements in front of a row's first 16-byte boundary.
@@ -133,54 +114,81 @@ __device__ __forceinline__ Raw8<T> raw_neg_inf() {
   return r;
 }
 
-// Maximum and sum of exponentials of one thread's share of p[0, n): threads `tid` of `nt`, and
-// the vectors [v0, v1) of the row's; the ends that no vector covers go to `ends`.
+// The largest of a thread's vectors; NaN is left out here and comes through the sum. 16-bit types two at a time.
 template <typename T>
-__device__ __forceinline__ void scan_row(const T* p, int n, int head, int v0, int v1, int tid, int nt, bool ends,
-                                         float& m, float& s) {
-  m = -INFINITY;
-  s = 0.f;
-  const T* body = p + head;
+__device__ __forceinline__ float max_of(const Raw8<T> (&raw)[kUnroll]) {
+  if constexpr (sizeof(T) == 4) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      float f[8];
+      unpack8<T>(raw[u], f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) mx = fmaxf(mx, f[k]);
+    }
+    return mx;
+  } else {
+    using T2 = std::conditional_t<std::is_same<T, __nv_bfloat16>::value, __nv_bfloat162, __half2>;
+    T2 mx = reinterpret_cast<const T2&>(raw[0].w[0].x);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const uint4& w = raw[u].w[0];
+      mx = __hmax2(__hmax2(mx, __hmax2(reinterpret_cast<const T2&>(w.x), reinterpret_cast<const T2&>(w.y))),
+                   __hmax2(reinterpret_cast<const T2&>(w.z), reinterpret_cast<const T2&>(w.w)));
+    }
+    const float lo = to_float(mx.x), hi = to_float(mx.y);
+    return fmaxf(fmaxf(-INFINITY, lo), hi);
+  }
+}
+
+// Adds kUnroll vectors of a thread to its maximum and sum.
+template <typename T>
+__device__ __forceinline__ void scan_vectors(const Raw8<T> (&raw)[kUnroll], float& m, float& s) {
+  const float mx = fmaxf(m, max_of<T>(raw)), a = anchor(mx);
+  if (mx != m) s *= expf(m - a);
+  m = mx;
+  const F2 neg = f2(-a, -a), c = f2(kLog2e, kLog2e), rest = f2(kLog2eRest, kLog2eRest);
+  F2 sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    F2 v[4];
+    unpack_f2<T>(raw[u], v);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const F2 t = v[k] + neg;
+      // what the constant loses in 32 bits is 1.3e-8 of the product, always to the same side: see finish_row
+      sum[k & 1] = sum[k & 1] + ex2(fma2(t, c, t * rest));
+    }
+  }
+  const float2 x = f2_values(sum[0] + sum[1]);
+  s += x.x + x.y;
+}
+
+// Calls use(raw, base) for the vectors [v0, v1) of p, of which thread `tid` of `nt` takes every nt-th: kUnroll of them at a
+// time, at base, base + nt ... (-inf beyond v1).
+template <typename T, typename F>
+__device__ __forceinline__ void stream_row(const T* p, int v0, int v1, int tid, int nt, F&& use) {
   for (int base = v0 + tid; base < v1; base += nt * kUnroll) {
     Raw8<T> raw[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const int v = base + u * nt;
-      raw[u] = v < v1 ? load_raw8<T>(body + (long long)v * 8) : raw_neg_inf<T>();
+      raw[u] = v < v1 ? load_raw8<T>(p + (long long)v * 8) : raw_neg_inf<T>();
     }
-    float f[kUnroll][8], mx = m;
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      unpack8<T>(raw[u], f[u]);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) mx = fmaxf(mx, f[u][k]);
-    }
-    const float a = anchor(mx);
-    float part[kUnroll];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-#pragma unroll
-      for (int k = 0; k < 8; k += 2) scaled2<true>(f[u][k], f[u][k + 1], -a);
-      float e0 = ex2(f[u][0]), e1 = ex2(f[u][1]);
-#pragma unroll
-      for (int k = 2; k < 8; k += 2) {
-        e0 += ex2(f[u][k]);
-        e1 += ex2(f[u][k + 1]);
-      }
-      part[u] = e0 + e1;
-    }
-    s = s * expf(m - a) + ((part[0] + part[1]) + (part[2] + part[3]));
-    m = mx;
-  }
-  if (ends) {
-    const int tail = head + (n - head) / 8 * 8;
-    for (int j = tid; j < head + (n - tail); j += nt) join(m, s, to_float(p[j < head ? j : tail + j - head]), 1.f);
+    use(raw, base);
   }
 }
 
-// What one thread does once a row's maximum and sum are known.
+// The values that no vector covers: `head` in front, and those behind the last of `vecs` vectors.
+template <typename T>
+__device__ __forceinline__ void scan_ends(const T* p, int n, int head, int vecs, int tid, int nt, float& m, float& s) {
+  const int tail = head + vecs * 8;
+  for (int j = tid; j < head + (n - tail); j += nt) join(m, s, to_float(p[j < head ? j : tail + j - head]), 1.f);
+}
+
+// What one thread does once a row's maximum and sum are known. Returns the derivative of the loss by logp, for kPolicy.
 template <Mode MODE>
-__device__ __forceinline__ void finish_row(const RowArgs& a, int row, float xy, float m, float s) {
+__device__ __forceinline__ float finish_row(const RowArgs& a, int row, float xy, float m, float s) {
   // ex2.approx comes out low on average: by 2e-8 of its value above 1/2 and by 5e-8 in every octave below (measured). One
   // token does not show it, but a sequence's sum of a thousand log-probabilities does. A thread takes its exponentials
   // against its own maximum, so that most of its sum is near 1: 2e-8 is what a row's sum is low by. The maximum is exact.
@@ -205,9 +213,12 @@ __device__ __forceinline__ void finish_row(const RowArgs& a, int row, float xy, 
     a.row_loss[row] = (float)loss;
     a.row_kl[row] = (float)kl;
     a.row_clipped[row] = clipped;
+    coef *= a.count ? (*a.count > 0 ? 1.0 / *a.count : 0.0) : 1.0 / a.rows;
     a.coef[row] = (float)coef;
+    return (float)coef;
   }
   if constexpr (MODE == kPreference) a.row_diff[row] = lp - (double)a.ref_logp[row];
+  return 0.f;
 }
 
 template <Mode MODE>
@@ -224,8 +235,7 @@ __device__ __forceinline__ void skip_row(const RowArgs& a, int row) {
 }
 
 template <typename T>
-__device__ __forceinline__ float target_logit(const RowArgs& a, const T* p, int row) {
-  const int64_t y = a.targets[row];
+__device__ __forceinline__ float target_logit(const RowArgs& a, const T* p, int64_t y) {
   if (y < 0 || y >= a.vocab) {
     atomicExch(a.error, (int)kErrBadIndex);
     return NAN;
@@ -244,50 +254,134 @@ __global__ void __launch_bounds__(32 * kWarpRows) warp_row_kernel(const RowArgs 
   }
   const T* p = row_of<T>(a.logits, a.stride_b, a.stride_s, a.seq, row);
   const int head = head_of(p, a.vocab);
-  const float xy = lane == 0 ? target_logit(a, p, row) : 0.f;
-  float m, s;
-  scan_row<T>(p, a.vocab, head, 0, (a.vocab - head) / 8, lane, 32, true, m, s);
+  const float xy = lane == 0 ? target_logit(a, p, a.targets[row]) : 0.f;
+  const int vecs = (a.vocab - head) / 8;
+  float m = -INFINITY, s = 0.f;
+  stream_row<T>(p + head, 0, vecs, lane, 32, [&](const Raw8<T>(&raw)[kUnroll], int) { scan_vectors<T>(raw, m, s); });
+  scan_ends<T>(p, a.vocab, head, vecs, lane, 32, m, s);
   warp_join(m, s);
   if (lane == 0) finish_row<MODE>(a, row, xy, m, s);
 }
 
-// One cluster of CTAs per row (often a cluster of one). With fewer rows than the GPU has room for, a row is
-// split over the cluster's CTAs, which hand their maximum and sum to the first one's shared memory.
-template <typename T, Mode MODE>
-__global__ void __launch_bounds__(kRowThreads) row_kernel(const RowArgs a) {
-  __shared__ float2 warps[kRowThreads / 32];
+// Gradient of one vector; `hot` is the target's place in it, if it has one in 0..7.
+template <typename T>
+__device__ __forceinline__ void grad_vector(const Raw8<T>& raw, T* to, bool aligned, float m, float neg, int hot, float c) {
+  const F2 minus = f2(-m, -m), scale = f2(kLog2e, kLog2e), factor = f2(neg, neg);
+  F2 f[4];
+  unpack_f2<T>(raw, f);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) f[k] = factor * ex2((f[k] + minus) * scale);
+  if ((unsigned)hot < 8u) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f[k] = f[k] + f2(2 * k == hot ? c : 0.f, 2 * k + 1 == hot ? c : 0.f);
+  }
+  const Raw8<T> out = pack_f2<T>(f);
+  if (aligned) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(to)[i] = out.w[i];
+  } else {  // the gradient's rows lie on other boundaries than the logits'
+#pragma unroll
+    for (int k = 0; k < 8; ++k) to[k] = reinterpret_cast<const T*>(&out)[k];
+  }
+}
+
+// The ends that no vector covers.
+template <typename T>
+__device__ __forceinline__ void grad_ends(const T* p, T* g, int n, int head, int vecs, int tid, int nt, float m, float neg,
+                                          int y, float c) {
+  const int tail = head + vecs * 8;
+  for (int i = tid; i < head + (n - tail); i += nt) {
+    const int j = i < head ? i : tail + i - head;
+    g[j] = from_float<T>(fmaf(neg, ex2((to_float(p[j]) - m) * kLog2e), j == y ? c : 0.f));
+  }
+}
+
+// Zeros in a share of g[0, n).
+template <typename T>
+__device__ __forceinline__ void fill_zero(T* g, int n, int share, int shares, int tid, int nt) {
+  const int head = head_of(g, n), vecs = (n - head) / 8, tail = head + vecs * 8;
+  const float zero[8] = {};
+  const int each = ((unsigned)vecs + shares - 1) / (unsigned)shares, v1 = min((share + 1) * each, vecs);
+  for (int v = share * each + tid; v < v1; v += nt) store8t<T>(g + head + (long long)v * 8, zero);
+  if (share == 0)
+    for (int j = tid; j < head + (n - tail); j += nt) g[j < head ? j : tail + j - head] = from_float<T>(0.f);
+}
+
+// Gradient of the vectors [v0, v1) of p.
+template <typename T>
+__device__ __forceinline__ void grad_row(const T* p, T* g, int v0, int v1, int tid, int nt, float m, float neg, int hot, float c) {
+  const bool aligned = (reinterpret_cast<uintptr_t>(g) & 15) == 0;
+  stream_row<T>(p, v0, v1, tid, nt, [&](const Raw8<T>(&raw)[kUnroll], int base) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int v = base + u * nt;
+      if (v < v1) grad_vector<T>(raw[u], g + (long long)v * 8, aligned, m, neg, hot - v * 8, c);
+    }
+  });
+}
+
+constexpr int kRowThreads = 256;
+constexpr int kGradRowThreads = 256;
+constexpr int kGradPart = 80 * 1024;
+
+// A cluster of CTAs per row, most often of one: with fewer rows than the GPU has room for a row is split, and the parts are
+// joined through the first CTA's shared memory. With GRAD the row's gradient follows at once, while the row is in the L2.
+template <typename T, Mode MODE, bool GRAD, int NT>
+__global__ void __launch_bounds__(NT) row_kernel(const RowArgs a) {
+  __shared__ float2 warps[NT / 32];
   __shared__ float2 parts[8];  // of the cluster's CTAs, in the first one
+  __shared__ float3 known;     // m, -c / s and c, for GRAD
   cg::cluster_group cluster = cg::this_cluster();
-  const int split = cluster.num_blocks(), rank = cluster.block_rank();
+  const unsigned split = cluster.num_blocks();
+  const int rank = cluster.block_rank(), tid = threadIdx.x;
   const int row = blockIdx.x / split;
+  T* g = GRAD ? static_cast<T*>(a.grad) + (long long)row * a.vocab : nullptr;
   if (a.mask && !a.mask[row]) {  // the whole cluster leaves
-    if (rank == 0 && threadIdx.x == 0) skip_row<MODE>(a, row);
+    if (GRAD) fill_zero<T>(g, a.vocab, rank, split, tid, NT);
+    if (rank == 0 && tid == 0) skip_row<MODE>(a, row);
     return;
   }
   if (split > 1) cluster.barrier_arrive();  // waited for below: all have begun before one writes to another
   const T* p = row_of<T>(a.logits, a.stride_b, a.stride_s, a.seq, row);
   const int head = head_of(p, a.vocab), vecs = (a.vocab - head) / 8;
-  const float xy = rank == 0 && threadIdx.x == 0 ? target_logit(a, p, row) : 0.f;
-  float m, s;
-  scan_row<T>(p, a.vocab, head, (int)((long long)vecs * rank / split), (int)((long long)vecs * (rank + 1) / split),
-              threadIdx.x, kRowThreads, rank == 0, m, s);
+  const int each = (vecs + split - 1) / split, v0 = min(rank * each, vecs), v1 = min(v0 + each, vecs);
+  const int64_t y = a.targets[row];  // looked at once the row has been read
+  float m = -INFINITY, s = 0.f;
+  stream_row<T>(p + head, v0, v1, tid, NT, [&](const Raw8<T>(&raw)[kUnroll], int) { scan_vectors<T>(raw, m, s); });
+  if (rank == 0) scan_ends<T>(p, a.vocab, head, vecs, tid, NT, m, s);
   warp_join(m, s);
-  if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = make_float2(m, s);
+  if ((tid & 31) == 0) warps[tid >> 5] = make_float2(m, s);
   __syncthreads();
-  if (threadIdx.x < 32) {
-    const float2 w = threadIdx.x < kRowThreads / 32 ? warps[threadIdx.x] : make_float2(-INFINITY, 0.f);
+  if (tid < 32) {
+    const float2 w = tid < NT / 32 ? warps[tid] : make_float2(-INFINITY, 0.f);
     m = w.x;
     s = w.y;
     warp_join(m, s);
   }
   if (split > 1) {
     cluster.barrier_wait();
-    if (threadIdx.x == 0) *cluster.map_shared_rank(&parts[rank], 0) = make_float2(m, s);
+    if (tid == 0) *cluster.map_shared_rank(&parts[rank], 0) = make_float2(m, s);
     cluster.sync();
-    if (rank == 0 && threadIdx.x == 0)
-      for (int i = 1; i < split; ++i) join(m, s, parts[i].x, parts[i].y);
+    if (rank == 0 && tid == 0)
+      for (int i = 1; i < (int)split; ++i) join(m, s, parts[i].x, parts[i].y);
   }
-  if (rank == 0 && threadIdx.x == 0) finish_row<MODE>(a, row, xy, m, s);
+  if (rank == 0 && tid == 0) {
+    const float c = finish_row<MODE>(a, row, target_logit(a, p, y), m, s);
+    if constexpr (GRAD)
+      for (int i = 0; i < (int)split; ++i) *cluster.map_shared_rank(&known, i) = make_float3(anchor(m), -c / s, c);
+  }
+  if constexpr (GRAD) {
+    if (split > 1) cluster.sync();
+    else __syncthreads();
+    const float3 k = known;
+    if (k.z == 0.f) {
+      fill_zero<T>(g, a.vocab, rank, split, tid, NT);
+      return;
+    }
+    const int hot = y >= 0 && y < a.vocab ? (int)y - head : INT_MIN;
+    grad_row<T>(p + head, g + head, v0, v1, tid, NT, k.x, k.y, hot, k.z);
+    if (rank == 0) grad_ends<T>(p, g, a.vocab, head, vecs, tid, NT, k.x, k.y, (int)y, k.z);
+  }
 }
 
 struct GradArgs {
@@ -301,70 +395,34 @@ struct GradArgs {
   const float* scale;  // null: 1
   const float2* stats;
   void* grad;  // contiguous
+  bool ready;  // grad holds the gradient for a scale of 1 already
 };
 
 constexpr int kGradThreads = 256;
 
-// dx_j = c ([j == y] - exp(x_j - m) / s). Each CTA takes one of a row's `chunks`. Rows with c = 0 are not read.
+// dx_j = c ([j == y] - exp(x_j - m) / s). A CTA takes one of a row's `chunks` at a time. Rows with c = 0 are not read.
 template <typename T>
 __global__ void __launch_bounds__(kGradThreads) logprob_grad_kernel(const GradArgs a) {
-  const int row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
-  const int n = a.vocab;
-  T* g = static_cast<T*>(a.grad) + (long long)row * n;
-  float c = a.mask && !a.mask[row] ? 0.f : a.coef[row / a.rows_per_coef];
-  if (c != 0.f && a.scale) c *= *a.scale;
-  const int g_head = head_of(g, n), vecs = (n - g_head) / 8;
-  const int v0 = (int)((long long)vecs * chunk / a.chunks), v1 = (int)((long long)vecs * (chunk + 1) / a.chunks);
-  const int tail = g_head + vecs * 8;
-  if (c == 0.f) {
-    const float zero[8] = {};
-    for (int v = v0 + threadIdx.x; v < v1; v += kGradThreads) store8t<T>(g + g_head + (long long)v * 8, zero);
-    if (chunk == 0)
-      for (int j = threadIdx.x; j < g_head + (n - tail); j += kGradThreads)
-        g[j < g_head ? j : tail + j - g_head] = from_float<T>(0.f);
-    return;
-  }
-  const T* p = row_of<T>(a.logits, a.stride_b, a.stride_s, a.seq, row);
-  const float2 st = a.stats[row];
-  const float m = st.x, neg = -c / st.y;
-  const int y = (int)a.targets[row];
-  auto one = [&](int j) {
-    const float e = ex2((to_float(p[j]) - m) * kLog2e);
-    g[j] = from_float<T>(fmaf(neg, e, j == y ? c : 0.f));
-  };
-  if (((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0) {
-    const T *src = p + g_head;
-    T* dst = g + g_head;
-    const int yv = y >= g_head ? (y - g_head) / 8 : -1, yk = (y - g_head) & 7;
-    for (int base = v0 + threadIdx.x; base < v1; base += kGradThreads * kUnroll) {
-      Raw8<T> raw[kUnroll];
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int v = base + u * kGradThreads;
-        if (v < v1) raw[u] = load_raw8<T>(src + (long long)v * 8);
-      }
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int v = base + u * kGradThreads;
-        if (v >= v1) break;
-        float f[8];
-        unpack8<T>(raw[u], f);
-#pragma unroll
-        for (int k = 0; k < 8; k += 2) scaled2<false>(f[k], f[k + 1], -m);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) f[k] = neg * ex2(f[k]);
-        if (v == yv) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) f[k] += k == yk ? c : 0.f;
-        }
-        store8t<T>(dst + (long long)v * 8, f);
-      }
+  const float scale = a.scale ? *a.scale : 1.f;
+  if (a.ready && scale == 1.f) return;
+  for (unsigned unit = blockIdx.x; unit < (unsigned)a.rows * a.chunks; unit += gridDim.x) {
+    const int row = unit / (unsigned)a.chunks, chunk = unit - row * a.chunks;
+    T* g = static_cast<T*>(a.grad) + (long long)row * a.vocab;
+    float c = a.mask && !a.mask[row] ? 0.f : a.coef[(unsigned)row / (unsigned)a.rows_per_coef];
+    if (c != 0.f) c *= scale;
+    if (c == 0.f) {
+      fill_zero<T>(g, a.vocab, chunk, a.chunks, threadIdx.x, kGradThreads);
+      continue;
     }
-  } else {  // the gradient's rows lie on other boundaries than the logits'
-    for (int j = g_head + v0 * 8 + threadIdx.x; j < g_head + v1 * 8; j += kGradThreads) one(j);
+    const T* p = row_of<T>(a.logits, a.stride_b, a.stride_s, a.seq, row);
+    const int head = head_of(p, a.vocab), vecs = (a.vocab - head) / 8;
+    const int each = ((unsigned)vecs + a.chunks - 1) / (unsigned)a.chunks, v0 = chunk * each, v1 = min(v0 + each, vecs);
+    const float2 st = a.stats[row];
+    const int64_t y = a.targets[row];
+    const int hot = y >= 0 && y < a.vocab ? (int)y - head : INT_MIN;
+    grad_row<T>(p + head, g + head, v0, v1, threadIdx.x, kGradThreads, st.x, -c / st.y, hot, c);
+    if (chunk == 0) grad_ends<T>(p, g, a.vocab, head, vecs, threadIdx.x, kGradThreads, st.x, -c / st.y, (int)y, c);
   }
-  if (chunk == 0)
-    for (int j = threadIdx.x; j < g_head + (n - tail); j += kGradThreads) one(j < g_head ? j : tail + j - g_head);
 }
 
 constexpr int kReduceThreads = 1024;
@@ -382,28 +440,34 @@ __device__ __forceinline__ double block_sum(double v, double* smem) {
   return v;
 }
 
-// Means over the rows that count, and the rows' coefficients divided by their number. One CTA: the rows' values are
-// a vocabulary's size less than what the row kernel read.
+// Rows that the mask keeps.
+__global__ void __launch_bounds__(kReduceThreads) count_kernel(const bool* mask, int rows, int* count) {
+  __shared__ double smem[32];
+  double n = 0;
+  for (int i = threadIdx.x; i < rows; i += kReduceThreads) n += mask[i] ? 1 : 0;
+  n = block_sum(n, smem);
+  if (threadIdx.x == 0) *count = (int)n;
+}
+
+// Means over the rows that count. One CTA: the rows' values are a vocabulary's size less than what the row kernel read.
 __global__ void __launch_bounds__(kReduceThreads) policy_reduce_kernel(const RowArgs a, float* loss, float* kl, float* clipped) {
   __shared__ double smem[32];
-  double l = 0, d = 0, c = 0, n = 0;
+  double l = 0, d = 0, c = 0;
   for (int i = threadIdx.x; i < a.rows; i += kReduceThreads) {
     l += a.row_loss[i];
     d += a.row_kl[i];
     c += a.row_clipped[i] ? 1 : 0;
-    n += !a.mask || a.mask[i] ? 1 : 0;
   }
   l = block_sum(l, smem);
   d = block_sum(d, smem);
   c = block_sum(c, smem);
-  n = block_sum(n, smem);
-  const double inv = n > 0 ? 1.0 / n : 0.0;
   if (threadIdx.x == 0) {
+    const int n = a.count ? *a.count : a.rows;
+    const double inv = n > 0 ? 1.0 / n : 0.0;
     *loss = (float)(l * inv);
     *kl = (float)(d * inv);
     *clipped = (float)(c * inv);
   }
-  for (int i = threadIdx.x; i < a.rows; i += kReduceThreads) a.coef[i] = (float)(a.coef[i] * inv);
 }
 
 // A warp sums each sequence, then a thread takes each pair. coef[i] is the derivative by each of sequence i's logp.
@@ -478,11 +542,27 @@ at::Tensor row_values(const at::Tensor& v, const at::Tensor& targets, const char
   return v.contiguous();
 }
 
-// Rows up to this length go to a warp each: 8 vectors per lane. (A CTA's 512 threads would have less than one each.)
+// Rows up to this length go to a warp each: 8 vectors per lane. (A CTA's 256 threads would have one each.)
 constexpr int kWarpRowMax = 2048;
 
+bool in_warps(const Rows& r) { return r.vocab <= kWarpRowMax; }
+
+template <typename T, Mode MODE, bool GRAD, int NT>
+void launch_row_kernel(const RowArgs& a, int split, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)a.rows * split);
+  cfg.blockDim = dim3(NT);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim = {(unsigned)split, 1, 1};
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, row_kernel<T, MODE, GRAD, NT>, a));
+}
+
 template <Mode MODE>
-void launch_rows(const Rows& r, RowArgs a, cudaStream_t stream) {
+void launch_rows(const Rows& r, RowArgs& a, cudaStream_t stream) {
   a.logits = r.logits.const_data_ptr();
   a.stride_b = r.stride_b;
   a.stride_s = r.stride_s;
@@ -493,25 +573,22 @@ void launch_rows(const Rows& r, RowArgs a, cudaStream_t stream) {
   if (r.rows == 0) return;
   with_element(r.logits.scalar_type(), [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    if (r.vocab <= kWarpRowMax) {
+    if (in_warps(r)) {
       warp_row_kernel<T, MODE><<<(r.rows + kWarpRows - 1) / kWarpRows, 32 * kWarpRows, 0, stream>>>(a);
       C10_CUDA_KERNEL_LAUNCH_CHECK();
-    } else {
-      // Few rows: split each until every SM has two CTAs or a part is down to one round of its CTA's loads.
-      const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-      int split = 1;
-      while (split < 8 && (long long)r.rows * split < 2 * sms && r.vocab / split > 2 * kRowThreads * 8 * kUnroll) split *= 2;
-      cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3((unsigned)r.rows * split);
-      cfg.blockDim = dim3(kRowThreads);
-      cfg.stream = stream;
-      cudaLaunchAttribute attr;
-      attr.id = cudaLaunchAttributeClusterDimension;
-      attr.val.clusterDim = {(unsigned)split, 1, 1};
-      cfg.attrs = &attr;
-      cfg.numAttrs = 1;
-      C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, row_kernel<T, MODE>, a));
+      return;
     }
+    // Few rows: split each until every SM has two CTAs or a part is down to two rounds of its CTA's loads.
+    const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+    int split = 1;
+    while (split < 8 && (int64_t)r.rows * split < 2 * sms && r.vocab / split > 2 * kRowThreads * 8 * kUnroll) split *= 2;
+    if constexpr (MODE == kPolicy) {
+      if (a.grad) {
+        while (split < 8 && (int64_t)r.vocab * sizeof(T) / split > kGradPart) split *= 2;
+        return launch_row_kernel<T, MODE, true, kGradRowThreads>(a, split, stream);
+      }
+    }
+    launch_row_kernel<T, MODE, false, kRowThreads>(a, split, stream);
   });
   count_launches(1);
 }
@@ -538,6 +615,12 @@ std::tuple<at::Tensor, at::Tensor> token_logprobs_fwd(const at::Tensor& logits, 
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> policy_loss_fwd(
     const at::Tensor& logits, const at::Tensor& targets, const at::Tensor& old_logp, const at::Tensor& advantages,
     const OptTensor& ref_logp, const OptTensor& mask, double clip_low, double clip_high, double kl_coef) {
+  return policy_loss_fwd_grad(logits, targets, old_logp, advantages, ref_logp, mask, clip_low, clip_high, kl_coef, nullptr);
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> policy_loss_fwd_grad(
+    const at::Tensor& logits, const at::Tensor& targets, const at::Tensor& old_logp, const at::Tensor& advantages,
+    const OptTensor& ref_logp, const OptTensor& mask, double clip_low, double clip_high, double kl_coef, at::Tensor* grad) {
   const Rows r = rows_of(logits, targets, mask);
   TORCH_CHECK_VALUE(clip_low >= 0 && clip_low <= 1 && clip_high >= 0, "clip_low in [0, 1] and clip_high >= 0 expected, got ",
                     clip_low, " and ", clip_high);
@@ -550,7 +633,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
   const auto m = mask.has_value() ? mask->contiguous() : at::Tensor();
   auto loss = at::empty({}, f32), kl = at::empty({}, f32), clipped = at::empty({}, f32);
   auto logp = at::empty(targets.sizes(), f32), coef = at::empty(targets.sizes(), f32), stats = at::empty({r.rows, 2}, f32);
-  auto row = at::empty({2, r.rows}, f32), row_clipped = at::empty({r.rows}, f32.dtype(at::kBool));
+  // loss and KL of each row, whether it is clipped, and the number of rows that count
+  auto work = at::empty({2 * (int64_t)r.rows + 1 + (r.rows + 3) / 4}, f32);
   RowArgs a = {};
   a.targets = t.const_data_ptr<int64_t>();
   a.mask = m.defined() ? m.const_data_ptr<bool>() : nullptr;
@@ -562,13 +646,23 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
   a.clip_low = (float)clip_low;
   a.clip_high = (float)clip_high;
   a.kl_coef = (float)kl_coef;
-  a.row_loss = row.mutable_data_ptr<float>();
+  a.row_loss = work.mutable_data_ptr<float>();
   a.row_kl = a.row_loss + r.rows;
-  a.row_clipped = row_clipped.mutable_data_ptr<bool>();
+  int* count = reinterpret_cast<int*>(a.row_kl + r.rows);
+  a.row_clipped = reinterpret_cast<bool*>(count + 1);
   a.coef = coef.mutable_data_ptr<float>();
   const auto stream = at::cuda::getCurrentCUDAStream();
+  if (a.mask) {
+    a.count = count;
+    count_kernel<<<1, kReduceThreads, 0, stream>>>(a.mask, r.rows, count);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+    count_launches(1);
+  }
+  if (grad && r.rows > 0 && !in_warps(r)) {
+    *grad = at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
+    a.grad = grad->mutable_data_ptr();
+  }
   launch_rows<kPolicy>(r, a, stream);
-  a.rows = r.rows;
   policy_reduce_kernel<<<1, kReduceThreads, 0, stream>>>(a, loss.mutable_data_ptr<float>(), kl.mutable_data_ptr<float>(),
                                                         clipped.mutable_data_ptr<float>());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
@@ -611,6 +705,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> preferenc
 
 at::Tensor token_logprobs_bwd(const at::Tensor& coef, const OptTensor& scale, const at::Tensor& logits,
                               const at::Tensor& targets, const at::Tensor& stats, const OptTensor& mask) {
+  return token_logprobs_bwd_ready(coef, scale, logits, targets, stats, mask, at::Tensor());
+}
+
+at::Tensor token_logprobs_bwd_ready(const at::Tensor& coef, const OptTensor& scale, const at::Tensor& logits,
+                                    const at::Tensor& targets, const at::Tensor& stats, const OptTensor& mask,
+                                    const at::Tensor& ready) {
   const Rows r = rows_of(logits, targets, mask);
   TORCH_CHECK_VALUE(coef.scalar_type() == at::kFloat && coef.device() == logits.device() &&
                         (coef.sizes() == targets.sizes() || (targets.dim() == 2 && coef.dim() == 1 && coef.size(0) == targets.size(0))),
@@ -622,7 +722,10 @@ at::Tensor token_logprobs_bwd(const at::Tensor& coef, const OptTensor& scale, co
     TORCH_CHECK_VALUE(scale->scalar_type() == at::kFloat && scale->device() == logits.device() && scale->numel() == 1,
                       "scale: one float32 value expected");
   const c10::cuda::CUDAGuard guard(logits.device());
-  auto grad = at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
+  // A captured pass may be replayed with another scale, and then finds what the last one left: it computes all of it.
+  const bool use_ready = ready.defined() && scale.has_value() &&
+                         c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None;
+  auto grad = use_ready ? ready : at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
   if (r.rows == 0) return grad;
   const auto t = targets.contiguous(), cf = coef.contiguous();
   const auto m = mask.has_value() ? mask->contiguous() : at::Tensor();
@@ -644,9 +747,13 @@ at::Tensor token_logprobs_bwd(const at::Tensor& coef, const OptTensor& scale, co
   const int per = kGradThreads * 8 * kUnroll * 2;
   a.chunks = std::max(1, (r.vocab + per - 1) / per);
   TORCH_CHECK_VALUE((long long)a.chunks * r.rows < (1ll << 31), "logits: too many values for one call");
+  a.ready = use_ready;
+  // where there is likely nothing to do, no more CTAs than are resident
+  const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  const unsigned grid = use_ready ? std::min(a.chunks * r.rows, sms * 4) : a.chunks * r.rows;
   with_element(logits.scalar_type(), [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    logprob_grad_kernel<T><<<(unsigned)(a.chunks * r.rows), kGradThreads, 0, at::cuda::getCurrentCUDAStream()>>>(a);
+    logprob_grad_kernel<T><<<grid, kGradThreads, 0, at::cuda::getCurrentCUDAStream()>>>(a);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   });
   count_launches(1);

@@ -9,7 +9,9 @@
 // x, which the backward reads anyway). A row (one head of one token) lies on 8 to 32 lanes, eight
 // values each, so that a row's sum takes three to five shuffles and every access is 16 bytes. A
 // group of lanes keeps its token's cosines and sines in registers for several heads of that token.
-// Queries and keys share one launch. All of it is computed in fp32 and rounded once.
+// Queries and keys share one launch. All of it is computed in fp32 and rounded once. Unpacked
+// arithmetic would take longer than the memory: the first and the second values of a lane's four
+// rotated pairs lie in packed registers, two and two, so that nothing is shuffled between them.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
@@ -23,6 +25,17 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// n / d for n < 2^31 by a multiplication (Granlund and Montgomery): the kernels' rows are found by divisions that would
+// otherwise stand in front of every load.
+struct Divisor {
+  unsigned d, mul, shift;
+  explicit Divisor(unsigned by = 1) : d(by), mul(0), shift(0) {
+    while ((1ull << shift) < d) ++shift;
+    mul = (unsigned)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+  }
+  __device__ __forceinline__ unsigned div(unsigned n) const { return (__umulhi(n, mul) + n) >> shift; }
+};
+
 // One of q and k: [B, S, H, D] with the last stride 1 and every row on a 16-byte boundary.
 struct Heads {
   const void* x;
@@ -31,7 +44,8 @@ struct Heads {
   long long yb, ys, yh;
   void* out;  // contiguous: y forward, dx backward
   const void* weight;
-  int heads, chunks;  // a token's heads are split into `chunks` runs
+  int heads;
+  Divisor chunks;  // a token's heads are split into so many runs
 };
 
 struct Args {
@@ -40,18 +54,71 @@ struct Args {
   const void* positions;  // null: a token's place in its sequence
   bool wide_positions;    // int64, else int32
   int table;              // rows of cos and sin
-  int seq, dim;
+  Divisor seq;
+  int dim;
   unsigned tokens;
   float eps;
   int* error;
   float* partial;  // backward: [CTAs, 2, D], null where no weight needs a gradient
 };
 
-template <typename TW>
-__device__ __forceinline__ void load_weight(const void* w, int at, float (&v)[8]) {
-  const TW* p = static_cast<const TW*>(w) + at;  // a parameter may lie on any boundary
+// A lane's eight values as four rotated pairs: a holds the pairs' first values (x0, x2), (x4, x6), b their second ones.
+struct Pairs {
+  F2 a[2], b[2];
+};
+
+template <typename T>
+__device__ __forceinline__ Pairs to_pairs(const Raw8<T>& r) {
+  float v[8];
+  unpack8<T>(r, v);
+  Pairs p;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] = to_float(p[k]);
+  for (int i = 0; i < 2; ++i) {
+    p.a[i] = f2(v[4 * i], v[4 * i + 2]);
+    p.b[i] = f2(v[4 * i + 1], v[4 * i + 3]);
+  }
+  return p;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_pairs(T* to, const Pairs& p) {
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float2 a = f2_values(p.a[i]), b = f2_values(p.b[i]);
+    v[4 * i] = a.x;
+    v[4 * i + 1] = b.x;
+    v[4 * i + 2] = a.y;
+    v[4 * i + 3] = b.y;
+  }
+  store8t<T>(to, v);
+}
+
+__device__ __forceinline__ Pairs no_pairs() {
+  const F2 z = f2(0.f, 0.f);
+  return Pairs{{z, z}, {z, z}};
+}
+
+// sum of x y over the lane's values
+__device__ __forceinline__ float dot8(const Pairs& x, const Pairs& y) {
+  const F2 s = fma2(x.b[1], y.b[1], fma2(x.a[1], y.a[1], fma2(x.b[0], y.b[0], x.a[0] * y.a[0])));
+  const float2 v = f2_values(s);
+  return v.x + v.y;
+}
+
+struct Turn {
+  F2 cos[2], sin[2], minus[2];
+};
+
+// The rotation by the angle: first and second value of each pair; by the negated angle with sin and minus exchanged.
+__device__ __forceinline__ Pairs rotate(const Pairs& x, const F2 (&c)[2], const F2 (&s)[2], const F2 (&minus)[2]) {
+  Pairs y;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    y.a[i] = fma2(x.b[i], minus[i], x.a[i] * c[i]);
+    y.b[i] = fma2(x.a[i], s[i], x.b[i] * c[i]);
+  }
+  return y;
 }
 
 template <int LPR>
@@ -62,67 +129,65 @@ __device__ __forceinline__ float row_sum(float v) {
 }
 
 // The lane's four cosines and sines of a token. A position outside the table makes the token's rows NaN and is reported.
-__device__ __forceinline__ void load_turn(const Args& a, unsigned token, int s, int at, bool active, float (&c)[4], float (&sn)[4]) {
-  long long pos = s;
-  if (a.positions) pos = a.wide_positions ? static_cast<const int64_t*>(a.positions)[token] : static_cast<const int*>(a.positions)[token];
-  if (pos < 0 || pos >= a.table) {
-    atomicExch(a.error, (int)kErrBadIndex);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) c[k] = sn[k] = NAN;
-    return;
+__device__ __forceinline__ Turn load_turn(const Args& a, unsigned token, unsigned s, int at, bool active) {
+  float4 c = make_float4(0.f, 0.f, 0.f, 0.f), sn = c;
+  if (active) {
+    long long pos = s;
+    if (a.positions) pos = a.wide_positions ? static_cast<const int64_t*>(a.positions)[token] : static_cast<const int*>(a.positions)[token];
+    if (pos < 0 || pos >= a.table) {
+      atomicExch(a.error, (int)kErrBadIndex);
+      c = sn = make_float4(NAN, NAN, NAN, NAN);
+    } else {
+      const long long row = pos * (a.dim / 2) + at / 2;
+      c = __ldg(reinterpret_cast<const float4*>(a.cos + row));
+      sn = __ldg(reinterpret_cast<const float4*>(a.sin + row));
+    }
   }
-  if (!active) return;
-  const long long row = pos * (a.dim / 2) + at / 2;
-  const float4 cv = __ldg(reinterpret_cast<const float4*>(a.cos + row)), sv = __ldg(reinterpret_cast<const float4*>(a.sin + row));
-  c[0] = cv.x; c[1] = cv.y; c[2] = cv.z; c[3] = cv.w;
-  sn[0] = sv.x; sn[1] = sv.y; sn[2] = sv.z; sn[3] = sv.w;
+  return Turn{{f2(c.x, c.y), f2(c.z, c.w)}, {f2(sn.x, sn.y), f2(sn.z, sn.w)}, {f2(-sn.x, -sn.y), f2(-sn.z, -sn.w)}};
 }
 
 // A run of up to HPG heads of one token, by one group of LPR lanes.
 template <typename T, typename TW, int LPR, int HPG>
 __global__ void __launch_bounds__(kThreads) fwd_kernel(const Args a) {
-  const unsigned units_q = a.tokens * a.part[0].chunks, units = units_q + a.tokens * a.part[1].chunks;
+  const unsigned units_q = a.tokens * a.part[0].chunks.d, units = units_q + a.tokens * a.part[1].chunks.d;
   const unsigned group = blockIdx.x * (kThreads / LPR) + threadIdx.x / LPR;
   const int at = (threadIdx.x % LPR) * 8;
-  const bool in = group < units, active = in && at < a.dim;
-  const bool is_k = in && group >= units_q;
+  const bool active = group < units && at < a.dim;
+  const bool is_k = group >= units_q;
   const Heads& h = a.part[is_k];
-  const unsigned unit = in ? group - (is_k ? units_q : 0) : 0;
-  const unsigned token = unit / h.chunks, chunk = unit % h.chunks;
-  const int h0 = (int)(chunk * HPG), n = in ? min(HPG, h.heads - h0) : 0;
-  const long long b = token / a.seq, s = token % a.seq;
+  const unsigned unit = group < units ? group - (is_k ? units_q : 0) : 0;
+  const unsigned token = h.chunks.div(unit), chunk = unit - token * h.chunks.d;
+  const int h0 = (int)(chunk * HPG), n = active ? min(HPG, h.heads - h0) : 0;
+  const unsigned b = a.seq.div(token), s = token - b * a.seq.d;
   const T* x = static_cast<const T*>(h.x) + b * h.xb + s * h.xs + h0 * h.xh + at;
   T* out = static_cast<T*>(h.out) + ((long long)token * h.heads + h0) * a.dim + at;
   Raw8<T> raw[HPG];
 #pragma unroll
   for (int i = 0; i < HPG; ++i)
-    if (active && i < n) raw[i] = load_raw8<T>(x + i * h.xh);
-  float c[4] = {}, sn[4] = {}, w[8] = {};
-  if (in) load_turn(a, token, (int)s, at, active, c, sn);
-  if (active) load_weight<TW>(h.weight, at, w);
+    if (i < n) raw[i] = load_raw8<T>(x + i * h.xh);
+  const Turn turn = load_turn(a, token, s, at, active);
+  Pairs w = no_pairs();
+  if (active) w = to_pairs<TW>(load_raw8<TW>(static_cast<const TW*>(h.weight) + at));
   const float inv_dim = 1.f / a.dim;
 #pragma unroll
   for (int i = 0; i < HPG; ++i) {
-    float v[8] = {};
-    if (active && i < n) unpack8<T>(raw[i], v);
-    float ss = 0.f;
+    Pairs v = no_pairs();
+    if (i < n) v = to_pairs<T>(raw[i]);
+    const float r = rsqrtf(row_sum<LPR>(dot8(v, v)) * inv_dim + a.eps);
+    const F2 r2 = f2(r, r);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) ss = fmaf(v[k], v[k], ss);
-    const float r = rsqrtf(row_sum<LPR>(ss) * inv_dim + a.eps);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float n0 = v[2 * k] * r * w[2 * k], n1 = v[2 * k + 1] * r * w[2 * k + 1];
-      v[2 * k] = n0 * c[k] - n1 * sn[k];
-      v[2 * k + 1] = n0 * sn[k] + n1 * c[k];
+    for (int j = 0; j < 2; ++j) {
+      v.a[j] = v.a[j] * r2 * w.a[j];
+      v.b[j] = v.b[j] * r2 * w.b[j];
     }
-    if (active && i < n) store8t<T>(out + (long long)i * a.dim, v);
+    if (i < n) store_pairs<T>(out + (long long)i * a.dim, rotate(v, turn.cos, turn.sin, turn.minus));
   }
 }
 
 // Each group walks over runs of heads, first of the queries and then of the keys, and keeps its
 // share of the weights' gradients in registers. The CTA joins its groups' shares in a fixed order.
 template <typename T, typename TW, int LPR, int HPG>
-__global__ void __launch_bounds__(kThreads) bwd_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3) bwd_kernel(const Args a) {
   constexpr int kGroups = kThreads / LPR;
   const int at = (threadIdx.x % LPR) * 8;
   const bool lane_in = at < a.dim;
@@ -131,62 +196,64 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(const Args a) {
 #pragma unroll 1
   for (int part = 0; part < 2; ++part) {
     const Heads& h = a.part[part];
-    const unsigned units = a.tokens * h.chunks;
-    float w[8] = {}, dw[8] = {};
-    if (lane_in) load_weight<TW>(h.weight, at, w);
+    const unsigned units = a.tokens * h.chunks.d;
+    Pairs w = no_pairs(), dw = no_pairs();
+    if (lane_in) w = to_pairs<TW>(load_raw8<TW>(static_cast<const TW*>(h.weight) + at));
     for (unsigned base = blockIdx.x * kGroups; base < units; base += gridDim.x * kGroups) {
       const unsigned group = base + threadIdx.x / LPR;
-      const bool in = group < units, active = in && lane_in;
-      const unsigned unit = in ? group : 0;
-      const unsigned token = unit / h.chunks, chunk = unit % h.chunks;
-      const int h0 = (int)(chunk * HPG), n = in ? min(HPG, h.heads - h0) : 0;
-      const long long b = token / a.seq, s = token % a.seq;
+      const bool active = group < units && lane_in;
+      const unsigned unit = group < units ? group : 0;
+      const unsigned token = h.chunks.div(unit), chunk = unit - token * h.chunks.d;
+      const int h0 = (int)(chunk * HPG), n = active ? min(HPG, h.heads - h0) : 0;
+      const unsigned b = a.seq.div(token), s = token - b * a.seq.d;
       const T* x = static_cast<const T*>(h.x) + b * h.xb + s * h.xs + h0 * h.xh + at;
       const T* dy = static_cast<const T*>(h.dy) + b * h.yb + s * h.ys + h0 * h.yh + at;
       T* out = static_cast<T*>(h.out) + ((long long)token * h.heads + h0) * a.dim + at;
       Raw8<T> rx[HPG], ry[HPG];
 #pragma unroll
       for (int i = 0; i < HPG; ++i)
-        if (active && i < n) {
+        if (i < n) {
           rx[i] = load_raw8<T>(x + i * h.xh);
           ry[i] = load_raw8<T>(dy + i * h.yh);
         }
-      float c[4] = {}, sn[4] = {};
-      if (in) load_turn(a, token, (int)s, at, active, c, sn);
+      const Turn turn = load_turn(a, token, s, at, active);
 #pragma unroll
       for (int i = 0; i < HPG; ++i) {
-        float v[8] = {}, g[8] = {};
-        if (active && i < n) {
-          unpack8<T>(rx[i], v);
-          unpack8<T>(ry[i], g);
-        }
-        float ss = 0.f, dot = 0.f;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float g0 = g[2 * k] * c[k] + g[2 * k + 1] * sn[k], g1 = g[2 * k + 1] * c[k] - g[2 * k] * sn[k];
-          g[2 * k] = g0;
-          g[2 * k + 1] = g1;
+        Pairs v = no_pairs(), g = no_pairs(), u;
+        if (i < n) {
+          v = to_pairs<T>(rx[i]);
+          g = rotate(to_pairs<T>(ry[i]), turn.cos, turn.minus, turn.sin);
         }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          ss = fmaf(v[k], v[k], ss);
-          dot = fmaf(g[k] * w[k], v[k], dot);
+        for (int j = 0; j < 2; ++j) {
+          u.a[j] = g.a[j] * w.a[j];
+          u.b[j] = g.b[j] * w.b[j];
         }
-        ss = row_sum<LPR>(ss);
-        dot = row_sum<LPR>(dot);
-        const float r = rsqrtf(ss * inv_dim + a.eps), f = r * r * dot * inv_dim;
+        const float ss = row_sum<LPR>(dot8(v, v)), dot = row_sum<LPR>(dot8(u, v));
+        const float r = rsqrtf(ss * inv_dim + a.eps), f = -(r * r * dot * inv_dim) * r;
+        const F2 r2 = f2(r, r), ff = f2(f, f);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float xr = v[k] * r;
-          if (i < n) dw[k] = fmaf(g[k], xr, dw[k]);
-          v[k] = r * (g[k] * w[k] - v[k] * f);
+        for (int j = 0; j < 2; ++j) {
+          if (i < n) {
+            dw.a[j] = fma2(g.a[j], v.a[j] * r2, dw.a[j]);
+            dw.b[j] = fma2(g.b[j], v.b[j] * r2, dw.b[j]);
+          }
+          v.a[j] = fma2(u.a[j], r2, v.a[j] * ff);
+          v.b[j] = fma2(u.b[j], r2, v.b[j] * ff);
         }
-        if (active && i < n) store8t<T>(out + (long long)i * a.dim, v);
+        if (i < n) store_pairs<T>(out + (long long)i * a.dim, v);
       }
     }
     if (a.partial) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) share[threadIdx.x / LPR][at + k] = dw[k];
+      for (int j = 0; j < 2; ++j) {
+        const float2 p = f2_values(dw.a[j]), q = f2_values(dw.b[j]);
+        float* to = &share[threadIdx.x / LPR][at + 4 * j];
+        to[0] = p.x;
+        to[1] = q.x;
+        to[2] = p.y;
+        to[3] = q.y;
+      }
       __syncthreads();
       for (int j = threadIdx.x; j < a.dim; j += kThreads) {
         float sum = 0.f;
@@ -199,19 +266,19 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(const Args a) {
   }
 }
 
-// Sum of the CTAs' shares: 32 lanes for each of 8 columns... one warp per column, in a fixed order.
+// Sum of the CTAs' shares, in a fixed order: 32 threads for each of eight columns.
 template <typename TW>
 __global__ void __launch_bounds__(kThreads) weight_grad_kernel(const float* partial, int ctas, int dim, TW* dwq, TW* dwk) {
-  __shared__ float smem[8][33];
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
+  __shared__ float smem[32][9];
+  const int c = threadIdx.x & 7, col = blockIdx.x * 8 + c, slice = threadIdx.x >> 3;
   float sum = 0.f;
-  if (col < 2 * dim)
-    for (int i = slice; i < ctas; i += 8) sum += partial[(long long)i * 2 * dim + col];
-  smem[slice][threadIdx.x & 31] = sum;
+#pragma unroll 4
+  for (int i = slice; i < ctas; i += 32) sum += partial[(long long)i * 2 * dim + col];
+  smem[slice][c] = sum;
   __syncthreads();
-  if (slice == 0 && col < 2 * dim) {
+  if (slice == 0) {
 #pragma unroll
-    for (int i = 1; i < 8; ++i) sum += smem[i][threadIdx.x & 31];
+    for (int i = 1; i < 32; ++i) sum += smem[i][c];
     (col < dim ? dwq : dwk)[col < dim ? col : col - dim] = from_float<TW>(sum);
   }
 }
@@ -252,7 +319,7 @@ void check_heads(const at::Tensor& q, const at::Tensor& k, const at::Tensor& qw,
   TORCH_CHECK_VALUE(q.size(0) * q.size(1) * std::max(q.size(2), k.size(2)) < (1ll << 30), "q, k: at most 2^30 heads of tokens expected");
 }
 
-// A table on a 16-byte boundary (its rows are multiples of 16 bytes: head_dim is one of 8).
+// A table or weight on a 16-byte boundary (head_dim is a multiple of 8, so that its rows and vectors stay on one).
 at::Tensor table16(const at::Tensor& t) {
   const auto c = t.contiguous();
   return reinterpret_cast<uintptr_t>(c.const_data_ptr()) % 16 ? c.clone() : c;
@@ -270,8 +337,8 @@ Args args_of(Kept& t, const at::Tensor& q, const at::Tensor& k, const at::Tensor
   t.k = rows16(k);
   t.cos = table16(cos);
   t.sin = table16(sin);
-  t.qw = qw.contiguous();
-  t.kw = kw.contiguous();
+  t.qw = table16(qw);
+  t.kw = table16(kw);
   Args a = {};
   const at::Tensor* xs[2] = {&t.q, &t.k};
   const at::Tensor* ws[2] = {&t.qw, &t.kw};
@@ -283,7 +350,7 @@ Args args_of(Kept& t, const at::Tensor& q, const at::Tensor& k, const at::Tensor
     h.xh = xs[i]->stride(2);
     h.weight = ws[i]->const_data_ptr();
     h.heads = (int)xs[i]->size(2);
-    h.chunks = std::max(1, (h.heads + hpg - 1) / hpg);
+    h.chunks = Divisor(std::max(1, (h.heads + hpg - 1) / hpg));
   }
   a.cos = t.cos.const_data_ptr<float>();
   a.sin = t.sin.const_data_ptr<float>();
@@ -293,7 +360,7 @@ Args args_of(Kept& t, const at::Tensor& q, const at::Tensor& k, const at::Tensor
     a.positions = t.pos.const_data_ptr();
     a.wide_positions = t.pos.scalar_type() == at::kLong;
   }
-  a.seq = (int)std::max<int64_t>(1, q.size(1));
+  a.seq = Divisor((unsigned)std::max<int64_t>(1, q.size(1)));
   a.dim = (int)q.size(3);
   a.tokens = (unsigned)(q.size(0) * q.size(1));
   a.eps = (float)eps;
@@ -340,7 +407,7 @@ std::tuple<at::Tensor, at::Tensor> qk_norm_rope_fwd(const at::Tensor& q, const a
   Args a = args_of(t, q, k, q_weight, k_weight, cos, sin, positions, eps, hpg);
   a.part[0].out = qo.mutable_data_ptr();
   a.part[1].out = ko.mutable_data_ptr();
-  const int64_t units = (int64_t)a.tokens * (a.part[0].chunks + a.part[1].chunks);
+  const int64_t units = (int64_t)a.tokens * (a.part[0].chunks.d + a.part[1].chunks.d);
   with_types(q, q_weight, [&](auto* tt, auto* tw, auto lanes) {
     using T = std::remove_pointer_t<decltype(tt)>;
     using TW = std::remove_pointer_t<decltype(tw)>;
@@ -383,10 +450,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_bwd(
   }
   a.part[0].out = dq.mutable_data_ptr();
   a.part[1].out = dk.mutable_data_ptr();
-  const int64_t units = (int64_t)a.tokens * std::max(a.part[0].chunks, a.part[1].chunks);
+  const int64_t units = (int64_t)a.tokens * std::max(a.part[0].chunks.d, a.part[1].chunks.d);
   const int groups = kThreads / lanes_per_row(q.size(3));
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  const int ctas = (int)std::min<int64_t>((units + groups - 1) / groups, (int64_t)sms * 4);
+  const int resident = sms * (q.scalar_type() == at::kFloat ? 2 : 3);  // as the kernel's launch bounds
+  const int ctas = (int)std::min<int64_t>((units + groups - 1) / groups, resident);
   at::Tensor partial;
   if (weight_grads) {
     partial = at::empty({ctas, 2, q.size(3)}, q.options().dtype(at::kFloat));
@@ -401,7 +469,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_bwd(
     else bwd_kernel<T, TW, L, 1><<<ctas, kThreads, 0, stream>>>(a);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
     if (weight_grads) {
-      weight_grad_kernel<TW><<<(2 * a.dim + 31) / 32, kThreads, 0, stream>>>(
+      weight_grad_kernel<TW><<<2 * a.dim / 8, kThreads, 0, stream>>>(
           a.partial, ctas, a.dim, static_cast<TW*>(dwq.mutable_data_ptr()), static_cast<TW*>(dwk.mutable_data_ptr()));
       C10_CUDA_KERNEL_LAUNCH_CHECK();
     }

@@ -6,12 +6,12 @@
 //   balance = E / (N^2 k) sum_e c_e sum_t p_te   (1 where every expert gets the same),  z = 1/N sum_t lse_t^2
 //   dl = g (dg - g.dg) at the chosen + p (dbalance E / (N^2 k) (c_e - c.p) + dz 2/N lse)
 //
-// A row lies on 1 to 32 lanes, eight logits (16 bytes of a 16-bit type) or two or four times that
-// on each. The choice takes k rounds of a maximum over the row by (value, index). Every group of
-// lanes walks over rows and keeps its sums of p and its counts in registers; a CTA joins them in a
-// fixed order and writes one part, and a second kernel of one CTA sums the parts in 64 bits. So
-// there are no atomics, and a run gives the same bits each time. What bounds it: launches for small
-// batches, the k rounds for many experts; the logits are read once forward and once backward.
+// Up to 32 experts a row lies on one, two or four lanes, eight logits on each; above, on a warp, two to 16 logits on each
+// lane. The choice takes k rounds of a maximum over the row by (value, index); on a warp a round is one redux over
+// order-preserving integer keys and a ballot, and only the winner's lane looks through its logits. Every group of lanes
+// walks over rows and keeps its sums of p and its counts in registers; a CTA joins them in a fixed order and writes one
+// part, and a second kernel sums the parts in 64 bits. So nothing that is rounded is summed by atomics, and a run gives
+// the same bits each time. What bounds it: launches for small batches, the instructions of the k rounds for many experts.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
@@ -39,7 +39,7 @@ __device__ __forceinline__ float ex2(float x) {
 struct Args {
   const void* logits;
   long long stride;  // elements between rows
-  bool vec;          // rows of whole 16-byte words on 16-byte boundaries
+  bool vec, vec_out;  // logits, dlogits: rows of whole words, each lane's on its own boundary
   int tokens, experts, top_k;
   const bool* mask;  // null: every token counts
   // forward
@@ -48,6 +48,9 @@ struct Args {
   int64_t* counts;
   float* sum_p;  // [E + 1, CTAs]: sums of p, last the sum of lse^2
   int* sum_c;    // [E + 1, CTAs]: choices, last the tokens that count
+  double* total_p;  // [E + 1]
+  int* total_c;     // [E + 1]
+  unsigned* ticket;
   // backward
   const void* dgates;                // null: none
   const float *dbalance, *dz;        // null: none
@@ -104,6 +107,25 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 
 __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k == 0xFFFFFFFFu ? 0x7FC00000u : k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
+}
+
+// Sums the warps' shares, [kWarps, width + 1] in shared memory, and writes the CTA's part. The first CTA also resets the
+// ticket that route_join_kernel draws.
+__device__ __forceinline__ void write_part(const Args& a, const float* join_p, const int* join_c, int width) {
+  __syncthreads();
+  for (int e = threadIdx.x; e <= a.experts; e += kThreads) {
+    const int from = e < a.experts ? e : width;
+    float p = 0.f;
+    int c = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      p += join_p[w * (width + 1) + from];
+      c += join_c[w * (width + 1) + from];
+    }
+    a.sum_p[(long long)e * gridDim.x + blockIdx.x] = p;
+    a.sum_c[(long long)e * gridDim.x + blockIdx.x] = c;
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0;
 }
 
 template <typename T, int LPR, int VPL>
@@ -220,31 +242,149 @@ __global__ void __launch_bounds__(kThreads) route_kernel(const Args a) {
       join_c[warp * (kExperts + 1) + kExperts] = sum_n;
     }
   }
-  __syncthreads();
-  for (int e = threadIdx.x; e <= a.experts; e += kThreads) {
-    const int from = e < a.experts ? e : kExperts;
-    float p = 0.f;
-    int c = 0;
+  write_part(a, join_p, join_c, kExperts);
+}
+
+// ------------------------------------------------------------------ a warp per row
+
+// VPL logits next to each other on each lane: lane order is index order.
+template <typename T, int VPL>
+__device__ __forceinline__ void load_lane(const Args& a, int row, int lane, float (&x)[VPL]) {
+  const T* p = static_cast<const T*>(a.logits) + (long long)row * a.stride + lane * VPL;
+  if (a.vec) {  // whole: the row ends with a lane, and every lane's share is on its own boundary
+    constexpr int kBytes = VPL * sizeof(T) < 16 ? VPL * sizeof(T) : 16;
+    using W = std::conditional_t<kBytes == 16, uint4, std::conditional_t<kBytes == 8, uint2, uint32_t>>;
+    union {
+      W w[VPL * sizeof(T) / kBytes];
+      T t[VPL];
+    } u;
+    if (lane * VPL < a.experts) {
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      p += join_p[w * (kExperts + 1) + from];
-      c += join_c[w * (kExperts + 1) + from];
+      for (int i = 0; i < (int)(VPL * sizeof(T) / kBytes); ++i) u.w[i] = __ldg(reinterpret_cast<const W*>(p) + i);
     }
-    a.sum_p[(long long)e * gridDim.x + blockIdx.x] = p;
-    a.sum_c[(long long)e * gridDim.x + blockIdx.x] = c;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) x[j] = lane * VPL < a.experts ? to_float(u.t[j]) : -INFINITY;
+  } else {
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) x[j] = lane * VPL + j < a.experts ? to_float(p[j]) : -INFINITY;
   }
+}
+
+// Each lane first sorts its keys (by swaps of neighbours only, so that equal ones stay in order), and a round then takes the
+// largest head of the lanes' lists: one redux, one ballot, and the winner's list moves up. The next row's logits are on
+// their way meanwhile.
+template <typename T, int VPL>
+__global__ void __launch_bounds__(kThreads, VPL == 16 ? 2 : 4) route_warp_kernel(const Args a) {
+  constexpr int kExperts = 32 * VPL;
+  __shared__ float join_p[kWarps * (kExperts + 1)];
+  __shared__ int join_c[kWarps * (kExperts + 1)];
+  __shared__ uint2 stash[kWarps][kMaxTopK];  // a row's keys and experts by rank
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int* count = join_c + warp * (kExperts + 1);  // the warp's own
+  for (int e = lane; e < kExperts; e += 32) count[e] = 0;
+  __syncwarp();
+  float sum_p[VPL] = {}, sum_z = 0.f;
+  int sum_n = 0;
+  const int step = gridDim.x * kWarps;
+  int row = blockIdx.x * kWarps + warp;
+  float next[VPL];
+  bool next_valid = false;
+  auto fetch = [&](int r) {
+    if (r < a.tokens) {
+      next_valid = !a.mask || a.mask[r];
+      load_lane<T, VPL>(a, r, lane, next);
+    }
+  };
+  fetch(row);
+  for (; row < a.tokens; row += step) {
+    const bool valid = next_valid;
+    float x[VPL];
+    uint32_t key[VPL], order[VPL];
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+      x[j] = next[j];
+      key[j] = lane * VPL + j < a.experts ? order_key(x[j]) : 0u;
+      order[j] = j;
+    }
+    fetch(row + step);
+#pragma unroll
+    for (int i = 0; i < VPL - 1; ++i) {
+#pragma unroll
+      for (int j = VPL - 2; j >= i; --j) {
+        const bool swap = key[j + 1] > key[j];
+        const uint32_t hi = max(key[j], key[j + 1]), lo = min(key[j], key[j + 1]), t = order[j];
+        order[j] = swap ? order[j + 1] : t;
+        order[j + 1] = swap ? t : order[j + 1];
+        key[j] = hi;
+        key[j + 1] = lo;
+      }
+    }
+    uint64_t list = 0;  // the sorted keys' places, four bits each
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) list |= (uint64_t)order[j] << (4 * j);
+    for (int i = 0; i < a.top_k; ++i) {
+      const uint32_t top = __reduce_max_sync(~0u, key[0]);
+      if (__ffs(__ballot_sync(~0u, key[0] == top)) - 1 == lane) {  // the first lane of those that have it
+        stash[warp][i] = make_uint2(top, lane * VPL + ((uint32_t)list & 15u));
+        list >>= 4;
+#pragma unroll
+        for (int j = 0; j < VPL - 1; ++j) key[j] = key[j + 1];
+        key[VPL - 1] = 0;
+      }
+    }
+    __syncwarp();
+    // softmax over all experts; the row's maximum may be -inf
+    const float top = key_value(stash[warp][0].x), m = top == -INFINITY ? 0.f : top;
+    float s = 0.f, e = 0.f;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+      x[j] = ex2((x[j] - m) * kLog2e);
+      s += x[j];
+    }
+    const bool mine = lane < a.top_k;
+    const uint2 pick = stash[warp][lane];
+    if (mine) e = ex2((key_value(pick.x) - top) * kLog2e);
+    float total = e;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      s += __shfl_xor_sync(~0u, s, o);
+      total += __shfl_xor_sync(~0u, total, o);
+    }
+    if (mine) {
+      const long long out = (long long)row * a.top_k + lane;
+      static_cast<T*>(a.gates)[out] = from_float<T>(valid ? e / total : 0.f);
+      a.chosen[out] = pick.y;
+      if (valid) count[pick.y] += 1;  // a row's experts differ
+    }
+    if (valid) {
+      const float inv = 1.f / s, lse = m + __log2f(s) * kLn2;
+      sum_n += 1;
+      sum_z = fmaf(lse, lse, sum_z);
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) sum_p[j] = fmaf(x[j], inv, sum_p[j]);
+    }
+    __syncwarp();
+  }
+#pragma unroll
+  for (int j = 0; j < VPL; ++j) join_p[warp * (kExperts + 1) + lane * VPL + j] = sum_p[j];
+  if (lane == 0) {
+    join_p[warp * (kExperts + 1) + kExperts] = sum_z;
+    count[kExperts] = sum_n;
+  }
+  write_part(a, join_p, join_c, kExperts);
 }
 
 constexpr int kJoinThreads = 512;
 
-// A warp sums each expert's parts.
+// A warp sums each expert's parts; the CTA that is done last takes the products, in the experts' order.
 __global__ void __launch_bounds__(kJoinThreads) route_join_kernel(const Args a, int parts, float* balance, float* z) {
-  __shared__ double sum_p[kMaxExperts + 1];
-  __shared__ int sum_c[kMaxExperts + 1];
+  __shared__ bool last;
   const int lane = threadIdx.x & 31;
-  for (int e = threadIdx.x >> 5; e <= a.experts; e += kJoinThreads / 32) {
+  const int e = (blockIdx.x * kJoinThreads + threadIdx.x) >> 5;
+  if (e <= a.experts) {
     double p = 0;
     int c = 0;
+#pragma unroll 4
     for (int i = lane; i < parts; i += 32) {
       p += a.sum_p[(long long)e * parts + i];
       c += a.sum_c[(long long)e * parts + i];
@@ -255,21 +395,150 @@ __global__ void __launch_bounds__(kJoinThreads) route_join_kernel(const Args a, 
       c += __shfl_xor_sync(~0u, c, o);
     }
     if (lane == 0) {
-      sum_p[e] = p;
-      sum_c[e] = c;
+      a.total_p[e] = p;
+      a.total_c[e] = c;
+      if (e < a.experts) a.counts[e] = c;
+      __threadfence();
     }
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < a.experts; e += kJoinThreads) a.counts[e] = sum_c[e];
-  if (threadIdx.x < 32) {
-    double dot = 0;
-    for (int e = lane; e < a.experts; e += 32) dot += sum_p[e] * sum_c[e];
+  if (threadIdx.x == 0) {
+    last = gridDim.x == 1 || atomicAdd(a.ticket, 1u) == gridDim.x - 1;
+    __threadfence();
+  }
+  __syncthreads();
+  if (!last || threadIdx.x >= 32) return;
+  double dot = 0;
+  for (int i = lane; i < a.experts; i += 32) dot += __ldcg(a.total_p + i) * __ldcg(a.total_c + i);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(~0u, dot, o);
-    if (lane == 0) {
-      const double n = sum_c[a.experts];
-      *balance = n > 0 ? (float)(dot * a.experts / (n * n * a.top_k)) : 0.f;
-      *z = n > 0 ? (float)(sum_p[a.experts] / n) : 0.f;
+  for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(~0u, dot, o);
+  if (lane == 0) {
+    const double n = __ldcg(a.total_c + a.experts);
+    *balance = n > 0 ? (float)(dot * a.experts / (n * n * a.top_k)) : 0.f;
+    *z = n > 0 ? (float)(__ldcg(a.total_p + a.experts) / n) : 0.f;
+  }
+}
+
+// c_e / (N k) of each expert to shared memory, [0, width); returns the number of choices.
+__device__ __forceinline__ int load_share(const Args& a, float* share, int* choices, int width) {
+  if (threadIdx.x < 32) {
+    int n = 0;
+    for (int e = threadIdx.x; e < a.experts; e += 32) n += (int)a.counts[e];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(~0u, n, o);
+    if (threadIdx.x == 0) *choices = n;
+  }
+  __syncthreads();
+  const int n = *choices;
+  for (int e = threadIdx.x; e < width; e += kThreads)
+    share[e] = e < a.experts && n > 0 ? (float)((double)a.counts[e] / n) : 0.f;
+  __syncthreads();
+  return n;
+}
+
+template <typename T, int VPL>
+__global__ void __launch_bounds__(kThreads, VPL == 16 ? 2 : 4) route_warp_grad_kernel(const Args a) {
+  constexpr int kExperts = 32 * VPL;
+  __shared__ float share[kExperts];
+  __shared__ int choices;
+  // {dgate, 1} of the chosen experts of a warp's row, 0 elsewhere: each warp scatters to and gathers from its own
+  __shared__ __align__(16) float2 picks[kWarps][kExperts];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int e = threadIdx.x; e < kWarps * kExperts; e += kThreads) (&picks[0][0])[e] = make_float2(0.f, 0.f);
+  const int count = load_share(a, share, &choices, kExperts);
+  const float n = (float)(count / a.top_k);
+  const float by_balance = a.dbalance && count > 0 ? *a.dbalance * a.experts / n : 0.f;
+  const float by_z = a.dz && count > 0 ? *a.dz * 2.f / n : 0.f;
+  float part[VPL];
+#pragma unroll
+  for (int j = 0; j < VPL; ++j) part[j] = share[lane * VPL + j];
+  const int step = gridDim.x * kWarps;
+  int row = blockIdx.x * kWarps + warp;
+  float next[VPL], next_dg = 0.f;
+  int next_at = -1;
+  bool next_valid = false;
+  auto fetch = [&](int r) {
+    if (r >= a.tokens) return;
+    next_valid = !a.mask || a.mask[r];
+    load_lane<T, VPL>(a, r, lane, next);
+    if (a.dgates && lane < a.top_k) {
+      const int64_t e = a.chosen[(long long)r * a.top_k + lane];
+      next_dg = to_float(static_cast<const T*>(a.dgates)[(long long)r * a.top_k + lane]);
+      next_at = e >= 0 && e < a.experts ? (int)e : -1;
+    }
+  };
+  fetch(row);
+  for (; row < a.tokens; row += step) {
+    T* out = static_cast<T*>(a.dlogits) + (long long)row * a.experts + lane * VPL;
+    float x[VPL];
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) x[j] = next[j];
+    const int at = next_at;
+    const float mine = next_dg;
+    const bool valid = next_valid;
+    fetch(row + step);
+    if (valid) {
+      if (at >= 0) picks[warp][at] = make_float2(mine, 1.f);
+      float m = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) m = fmaxf(m, x[j]);
+      m = group_max<32>(m);
+      m = m == -INFINITY ? 0.f : m;
+      __syncwarp();
+      // the chosen ones have the same maximum, so that one exponential serves both softmaxes
+      float s = 0.f, s_top = 0.f, dot = 0.f, mix = 0.f, dg[VPL], in[VPL];
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) {
+        const float2 pick = picks[warp][lane * VPL + j];
+        dg[j] = pick.x;
+        in[j] = pick.y;
+        x[j] = ex2((x[j] - m) * kLog2e);
+        s += x[j];
+        mix = fmaf(part[j], x[j], mix);
+        if (in[j] != 0.f) {
+          s_top += x[j];
+          dot = fmaf(x[j], dg[j], dot);
+        }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        s += __shfl_xor_sync(~0u, s, o);
+        mix += __shfl_xor_sync(~0u, mix, o);
+        s_top += __shfl_xor_sync(~0u, s_top, o);
+        dot += __shfl_xor_sync(~0u, dot, o);
+      }
+      if (at >= 0) picks[warp][at] = make_float2(0.f, 0.f);  // every lane has read: the shuffles lie between
+      const float inv = 1.f / s, inv_top = 1.f / s_top;
+      const float all = by_z * (m + __log2f(s) * kLn2) - by_balance * (mix * inv);
+      dot *= inv_top;
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) {
+        float g = x[j] * inv * fmaf(by_balance, part[j], all);
+        if (in[j] != 0.f) g = fmaf(x[j] * inv_top, dg[j] - dot, g);
+        x[j] = g;
+      }
+      __syncwarp();
+    } else {
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) x[j] = 0.f;
+    }
+    if (a.vec_out) {
+      constexpr int kBytes = VPL * sizeof(T) < 16 ? VPL * sizeof(T) : 16;
+      using W = std::conditional_t<kBytes == 16, uint4, std::conditional_t<kBytes == 8, uint2, uint32_t>>;
+      union {
+        W w[VPL * sizeof(T) / kBytes];
+        T t[VPL];
+      } u;
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) u.t[j] = from_float<T>(x[j]);
+      if (lane * VPL < a.experts) {
+#pragma unroll
+        for (int i = 0; i < (int)(VPL * sizeof(T) / kBytes); ++i) reinterpret_cast<W*>(out)[i] = u.w[i];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < VPL; ++j)
+        if (lane * VPL + j < a.experts) out[j] = from_float<T>(x[j]);
     }
   }
 }
@@ -280,20 +549,10 @@ __global__ void __launch_bounds__(kThreads) route_grad_kernel(const Args a) {
   __shared__ float share[kExperts];  // c_e / (N k)
   __shared__ int choices;
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
-  if (threadIdx.x < 32) {
-    int n = 0;
-    for (int e = threadIdx.x; e < a.experts; e += 32) n += (int)a.counts[e];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(~0u, n, o);
-    if (threadIdx.x == 0) choices = n;
-  }
-  __syncthreads();
-  for (int e = threadIdx.x; e < kExperts; e += kThreads)
-    share[e] = e < a.experts && choices > 0 ? (float)((double)a.counts[e] / choices) : 0.f;
-  __syncthreads();
-  const float n = (float)(choices / a.top_k);
-  const float by_balance = a.dbalance && choices > 0 ? *a.dbalance * a.experts / n : 0.f;
-  const float by_z = a.dz && choices > 0 ? *a.dz * 2.f / n : 0.f;
+  const int count = load_share(a, share, &choices, kExperts);
+  const float n = (float)(count / a.top_k);
+  const float by_balance = a.dbalance && count > 0 ? *a.dbalance * a.experts / n : 0.f;
+  const float by_z = a.dz && count > 0 ? *a.dz * 2.f / n : 0.f;
   for (int base = blockIdx.x * kGroups; base < a.tokens; base += gridDim.x * kGroups) {
     const int row = base + group;
     const bool in = row < a.tokens;
@@ -351,7 +610,7 @@ __global__ void __launch_bounds__(kThreads) route_grad_kernel(const Args a) {
         if ((picked >> (j + k)) & 1) g = fmaf(x[j + k] * inv_top, dg[j + k] - dot, g);
         v[k] = valid ? g : 0.f;
       }
-      if (a.experts % 8 == 0) {
+      if (a.vec_out) {
         if (e < a.experts) store8t<T>(out + e, v);
       } else {
 #pragma unroll
@@ -364,7 +623,9 @@ __global__ void __launch_bounds__(kThreads) route_grad_kernel(const Args a) {
 
 // ------------------------------------------------------------------ host
 
-// f(T, LPR, VPL): as few lanes per row as hold it at eight values each, then more values.
+// f(T, LPR, VPL): up to 32 experts as few lanes per row as hold it at eight logits each (a warp has eight rows or more
+// at once), above a warp per row, with as few logits per lane as hold it. (The lanes' form at 128 fp32 experts, top 8:
+// 56 us for 65535 rows against 20 us for the warp's.)
 template <typename F>
 void with_layout(const at::Tensor& logits, F&& f) {
   with_element(logits.scalar_type(), [&](auto* t) {
@@ -373,11 +634,20 @@ void with_layout(const at::Tensor& logits, F&& f) {
     if (e <= 8) f(t, integral_constant<int, 1>(), integral_constant<int, 8>());
     else if (e <= 16) f(t, integral_constant<int, 2>(), integral_constant<int, 8>());
     else if (e <= 32) f(t, integral_constant<int, 4>(), integral_constant<int, 8>());
-    else if (e <= 64) f(t, integral_constant<int, 8>(), integral_constant<int, 8>());
-    else if (e <= 128) f(t, integral_constant<int, 16>(), integral_constant<int, 8>());
+    else if (e <= 64) f(t, integral_constant<int, 32>(), integral_constant<int, 2>());
+    else if (e <= 128) f(t, integral_constant<int, 32>(), integral_constant<int, 4>());
     else if (e <= 256) f(t, integral_constant<int, 32>(), integral_constant<int, 8>());
     else f(t, integral_constant<int, 32>(), integral_constant<int, 16>());
   });
+}
+
+// Values that a lane has next to each other.
+int per_lane(int experts) { return experts <= 32 ? 8 : experts <= 64 ? 2 : experts <= 128 ? 4 : experts <= 256 ? 8 : 16; }
+
+// Whether rows `stride` elements apart can be moved in a lane's whole words, of up to 16 bytes.
+bool whole_words(const void* p, int64_t rows, int64_t stride, int experts, int64_t size) {
+  const int64_t word = std::min<int64_t>(16, per_lane(experts) * size);
+  return experts % per_lane(experts) == 0 && (rows <= 1 || stride * size % word == 0) && reinterpret_cast<uintptr_t>(p) % word == 0;
 }
 
 void check_route(const at::Tensor& logits, int64_t top_k, const OptTensor& mask) {
@@ -399,8 +669,7 @@ Args args_of(const at::Tensor& logits, const at::Tensor& mask, int64_t top_k) {
   a.tokens = (int)logits.size(0);
   a.experts = (int)logits.size(1);
   a.top_k = (int)top_k;
-  a.vec = a.experts % 8 == 0 && (a.tokens <= 1 || a.stride * logits.element_size() % 16 == 0) &&
-          reinterpret_cast<uintptr_t>(a.logits) % 16 == 0;
+  a.vec = whole_words(a.logits, a.tokens, a.stride, a.experts, logits.element_size());
   a.mask = mask.defined() ? mask.const_data_ptr<bool>() : nullptr;
   return a;
 }
@@ -418,6 +687,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> route_fwd
   auto gates = at::empty({t, top_k}, logits.options().memory_format(at::MemoryFormat::Contiguous));
   auto chosen = at::empty({t, top_k}, i64), counts = at::empty({e}, i64);
   auto balance = at::empty({}, f32), z = at::empty({}, f32);
+  if (t == 0) return {gates, chosen, counts.zero_(), balance.zero_(), z.zero_()};
   Args a = args_of(x, m, top_k);
   a.gates = gates.mutable_data_ptr();
   a.chosen = chosen.mutable_data_ptr<int64_t>();
@@ -426,20 +696,24 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> route_fwd
   with_layout(x, [&](auto* tag, auto lanes, auto values) {
     using T = std::remove_pointer_t<decltype(tag)>;
     constexpr int L = decltype(lanes)::value, V = decltype(values)::value;
-    const int groups = kThreads / L;
+    const int groups = kThreads / L;  // rows of a CTA at once
     const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
     const int ctas = (int)std::min<int64_t>((t + groups - 1) / groups, (int64_t)sms * 4);
-    auto part_p = at::empty({e + 1, ctas}, f32), part_c = at::empty({e + 1, ctas}, f32.dtype(at::kInt));
-    a.sum_p = part_p.template mutable_data_ptr<float>();
-    a.sum_c = part_c.template mutable_data_ptr<int>();
-    if (ctas) {
-      route_kernel<T, L, V><<<ctas, kThreads, 0, stream>>>(a);
-      C10_CUDA_KERNEL_LAUNCH_CHECK();
-    }
-    route_join_kernel<<<1, kJoinThreads, 0, stream>>>(a, ctas, balance.template mutable_data_ptr<float>(),
+    // one workspace: the CTAs' parts, the totals and the ticket
+    auto work = at::empty({(e + 1) * (2 * (int64_t)ctas + 3) + 2}, f32);
+    a.total_p = reinterpret_cast<double*>(work.template mutable_data_ptr<float>());
+    a.total_c = reinterpret_cast<int*>(a.total_p + e + 1);
+    a.ticket = reinterpret_cast<unsigned*>(a.total_c + e + 1);
+    a.sum_p = reinterpret_cast<float*>(a.ticket + 2);
+    a.sum_c = reinterpret_cast<int*>(a.sum_p + (e + 1) * ctas);
+    if constexpr (L == 32) route_warp_kernel<T, V><<<ctas, kThreads, 0, stream>>>(a);
+    else route_kernel<T, L, V><<<ctas, kThreads, 0, stream>>>(a);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+    const int joins = (int)((e + 1 + kJoinThreads / 32 - 1) / (kJoinThreads / 32));
+    route_join_kernel<<<joins, kJoinThreads, 0, stream>>>(a, ctas, balance.template mutable_data_ptr<float>(),
                                                       z.template mutable_data_ptr<float>());
     C10_CUDA_KERNEL_LAUNCH_CHECK();
-    count_launches(ctas ? 2 : 1);
+    count_launches(2);
   });
   return {gates, chosen, counts, balance, z};
 }
@@ -474,13 +748,16 @@ at::Tensor route_bwd(const OptTensor& dgates, const OptTensor& dbalance, const O
   a.dbalance = dbalance.has_value() ? dbalance->const_data_ptr<float>() : nullptr;
   a.dz = dz.has_value() ? dz->const_data_ptr<float>() : nullptr;
   a.dlogits = out.mutable_data_ptr();
+  a.vec_out = whole_words(a.dlogits, a.tokens, a.experts, a.experts, out.element_size());
   with_layout(x, [&](auto* tag, auto lanes, auto values) {
     using T = std::remove_pointer_t<decltype(tag)>;
     constexpr int L = decltype(lanes)::value, V = decltype(values)::value;
     const int groups = kThreads / L;
     const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-    const int ctas = (int)std::min<int64_t>((a.tokens + groups - 1) / groups, (int64_t)sms * 8);
-    route_grad_kernel<T, L, V><<<ctas, kThreads, 0, at::cuda::getCurrentCUDAStream()>>>(a);
+    const int ctas = (int)std::min<int64_t>((a.tokens + groups - 1) / groups, (int64_t)sms * (L == 32 ? 4 : 8));
+    const auto stream = at::cuda::getCurrentCUDAStream();
+    if constexpr (L == 32) route_warp_grad_kernel<T, V><<<ctas, kThreads, 0, stream>>>(a);
+    else route_grad_kernel<T, L, V><<<ctas, kThreads, 0, stream>>>(a);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   });
   count_launches(1);

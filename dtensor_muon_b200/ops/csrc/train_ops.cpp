@@ -2,6 +2,7 @@
 // gradients as autograd functions in C++ (a Python formula would cost more host time than the
 // small calls take). The schemas, the CPU and the fake kernels are in ops/library.py. Each
 // autograd function calls its operators through the dispatcher, so that tracers see them.
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
@@ -134,14 +135,22 @@ std::tuple<Tensor, Tensor> token_logprobs_autograd(const Tensor& logits, const T
   return {r[0], r[1]};
 }
 
+// A token's gradient needs nothing but that token's logp, so that the forward kernel can write the logits' gradient while
+// it has the row at hand, and the logits are read once instead of twice. It does so for a loss gradient of 1, which is
+// what backward() starts with; the backward pass then only looks at that value, and computes all of it where it is another.
+// The gradient is handed out once: a second backward pass of a retained graph computes its own. Not where a tracer or a
+// graph capture looks on, which would take the two passes apart.
 struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& targets, const Tensor& old_logp,
                                const Tensor& advantages, const OptTensor& ref_logp, const OptTensor& mask, double clip_low,
-                               double clip_high, double kl_coef) {
+                               double clip_high, double kl_coef, bool grad_now) {
     at::AutoDispatchBelowADInplaceOrView below;
     DMB_OP(op, "policy_loss", PolicyFwd);
+    Tensor grad;
     auto [loss, logp, kl, clipped, stats, coef] =
-        op.call(logits, targets, old_logp, advantages, ref_logp, mask, clip_low, clip_high, kl_coef);
+        grad_now ? policy_loss_fwd_grad(logits, targets, old_logp, advantages, ref_logp, mask, clip_low, clip_high, kl_coef, &grad)
+                 : op.call(logits, targets, old_logp, advantages, ref_logp, mask, clip_low, clip_high, kl_coef);
+    if (grad.defined()) ctx->saved_data["grad"] = grad;
     ctx->mark_non_differentiable({logp, kl, clipped, stats, coef});
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({logits, targets, stats, coef, saved(mask)});
@@ -149,10 +158,16 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     once("policy_loss");
-    variable_list out(9);
+    variable_list out(10);
     if (!g[0].defined()) return out;
     const auto s = ctx->get_saved_variables();
-    out[0] = logprob_grad(s[3], g[0], s[0], s[1], s[2], maybe(s[4]));
+    const auto ready = ctx->saved_data.find("grad");
+    if (ready == ctx->saved_data.end()) {
+      out[0] = logprob_grad(s[3], g[0], s[0], s[1], s[2], maybe(s[4]));
+    } else {
+      out[0] = token_logprobs_bwd_ready(s[3], g[0], s[0], s[1], s[2], maybe(s[4]), ready->second.toTensor());
+      ctx->saved_data.erase(ready);
+    }
     return out;
   }
 };
@@ -160,7 +175,11 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> policy_loss_autograd(
     const Tensor& logits, const Tensor& targets, const Tensor& old_logp, const Tensor& advantages, const OptTensor& ref_logp,
     const OptTensor& mask, double clip_low, double clip_high, double kl_coef) {
-  auto r = PolicyLoss::apply(logits, targets, old_logp, advantages, ref_logp, mask, clip_low, clip_high, kl_coef);
+  const auto keys = logits.key_set();
+  const bool plain = !keys.has(c10::DispatchKey::Python) && !keys.has(c10::DispatchKey::Functionalize);
+  const bool grad_now = plain && at::GradMode::is_enabled() && logits.requires_grad() &&
+                        c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None;
+  auto r = PolicyLoss::apply(logits, targets, old_logp, advantages, ref_logp, mask, clip_low, clip_high, kl_coef, grad_now);
   return {r[0], r[1], r[2], r[3], r[4], r[5]};
 }
 

@@ -36,10 +36,18 @@ std::tuple<at::Tensor, at::Tensor> token_logprobs_fwd(const at::Tensor& logits, 
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> policy_loss_fwd(
     const at::Tensor& logits, const at::Tensor& targets, const at::Tensor& old_logp, const at::Tensor& advantages,
     const OptTensor& ref_logp, const OptTensor& mask, double clip_low, double clip_high, double kl_coef);
+// As policy_loss_fwd; where the kernels can, they also put the logits' gradient for a loss gradient of 1 into *grad.
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> policy_loss_fwd_grad(
+    const at::Tensor& logits, const at::Tensor& targets, const at::Tensor& old_logp, const at::Tensor& advantages,
+    const OptTensor& ref_logp, const OptTensor& mask, double clip_low, double clip_high, double kl_coef, at::Tensor* grad);
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> preference_loss_fwd(
     const at::Tensor& logits, const at::Tensor& targets, const at::Tensor& ref_logp, const OptTensor& mask, double beta,
     double label_smoothing);
 at::Tensor token_logprobs_bwd(const at::Tensor& coef, const OptTensor& scale, const at::Tensor& logits,
                               const at::Tensor& targets, const at::Tensor& stats, const OptTensor& mask);
+// As token_logprobs_bwd; `ready`, where defined, holds the gradient for a scale of 1, and is returned with that for `scale`.
+at::Tensor token_logprobs_bwd_ready(const at::Tensor& coef, const OptTensor& scale, const at::Tensor& logits,
+                                    const at::Tensor& targets, const at::Tensor& stats, const OptTensor& mask,
+                                    const at::Tensor& ready);
 
 }  // namespace dmb

@@ -91,6 +91,58 @@ __device__ __forceinline__ void store8t(T* p, const float (&v)[8]) {  // p is 16
   for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = r.w[i];
 }
 
+// Two fp32 values in a 64-bit register: Blackwell's packed arithmetic does both in one instruction.
+struct F2 {
+  unsigned long long v;
+};
+
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 f2_values(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+// Eight values as four pairs of neighbours.
+template <typename T>
+__device__ __forceinline__ void unpack_f2(const Raw8<T>& r, F2 (&v)[4]) {
+  float f[8];
+  unpack8<T>(r, f);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = f2(f[2 * k], f[2 * k + 1]);
+}
+
+template <typename T>
+__device__ __forceinline__ Raw8<T> pack_f2(const F2 (&v)[4]) {
+  float f[8];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 x = f2_values(v[k]);
+    f[2 * k] = x.x;
+    f[2 * k + 1] = x.y;
+  }
+  return pack8<T>(f);
+}
+
 // Calls f with a null pointer of the element type of a tensor (fp32, bf16 or fp16).
 template <typename F>
 void with_element(at::ScalarType t, F&& f) {
