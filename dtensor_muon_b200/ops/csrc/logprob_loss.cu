@@ -599,8 +599,7 @@ std::tuple<at::Tensor, at::Tensor> token_logprobs_fwd(const at::Tensor& logits, 
                                                       const OptTensor& mask) {
   const Rows r = rows_of(logits, targets, mask);
   const c10::cuda::CUDAGuard guard(logits.device());
-  const auto f32 = logits.options().dtype(at::kFloat);
-  auto logp = at::empty(targets.sizes(), f32), stats = at::empty({r.rows, 2}, f32);
+  auto logp = new_empty(targets.sizes(), at::kFloat, logits), stats = new_empty({r.rows, 2}, at::kFloat, logits);
   const auto t = targets.contiguous();
   const auto m = mask.has_value() ? mask->contiguous() : at::Tensor();
   RowArgs a = {};
@@ -626,15 +625,14 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
                     clip_low, " and ", clip_high);
   TORCH_CHECK_VALUE(kl_coef == 0 || ref_logp.has_value(), "kl_coef needs ref_logp");
   const c10::cuda::CUDAGuard guard(logits.device());
-  const auto f32 = logits.options().dtype(at::kFloat);
   const auto t = targets.contiguous(), old = row_values(old_logp, targets, "old_logp"),
              adv = row_values(advantages, targets, "advantages");
   const auto ref = ref_logp.has_value() ? row_values(*ref_logp, targets, "ref_logp") : at::Tensor();
   const auto m = mask.has_value() ? mask->contiguous() : at::Tensor();
-  auto loss = at::empty({}, f32), kl = at::empty({}, f32), clipped = at::empty({}, f32);
-  auto logp = at::empty(targets.sizes(), f32), coef = at::empty(targets.sizes(), f32), stats = at::empty({r.rows, 2}, f32);
+  auto loss = new_empty({}, at::kFloat, logits), kl = new_empty({}, at::kFloat, logits), clipped = new_empty({}, at::kFloat, logits);
+  auto logp = new_empty(targets.sizes(), at::kFloat, logits), coef = new_empty(targets.sizes(), at::kFloat, logits), stats = new_empty({r.rows, 2}, at::kFloat, logits);
   // loss and KL of each row, whether it is clipped, and the number of rows that count
-  auto work = at::empty({2 * (int64_t)r.rows + 1 + (r.rows + 3) / 4}, f32);
+  auto work = new_empty({2 * (int64_t)r.rows + 1 + (r.rows + 3) / 4}, at::kFloat, logits);
   RowArgs a = {};
   a.targets = t.const_data_ptr<int64_t>();
   a.mask = m.defined() ? m.const_data_ptr<bool>() : nullptr;
@@ -659,7 +657,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
     count_launches(1);
   }
   if (grad && r.rows > 0 && !in_warps(r)) {
-    *grad = at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
+    *grad = new_empty(logits.sizes(), logits.scalar_type(), logits);
     a.grad = grad->mutable_data_ptr();
   }
   launch_rows<kPolicy>(r, a, stream);
@@ -679,13 +677,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> preferenc
   TORCH_CHECK_VALUE(beta > 0 && label_smoothing >= 0 && label_smoothing < 0.5,
                     "beta > 0 and label_smoothing in [0, 0.5) expected, got ", beta, " and ", label_smoothing);
   const c10::cuda::CUDAGuard guard(logits.device());
-  const auto f32 = logits.options().dtype(at::kFloat), f64 = logits.options().dtype(at::kDouble);
   const auto t = targets.contiguous(), ref = row_values(ref_logp, targets, "ref_logp");
   const auto m = mask.has_value() ? mask->contiguous() : at::Tensor();
   const int seqs = (int)targets.size(0), seq = (int)targets.size(1);
-  auto loss = at::empty({}, f32), rewards = at::empty({seqs}, f32), coef = at::empty({seqs}, f32);
-  auto logp = at::empty(targets.sizes(), f32), stats = at::empty({r.rows, 2}, f32);
-  auto wide = at::empty({r.rows + seqs}, f64);
+  auto loss = new_empty({}, at::kFloat, logits), rewards = new_empty({seqs}, at::kFloat, logits), coef = new_empty({seqs}, at::kFloat, logits);
+  auto logp = new_empty(targets.sizes(), at::kFloat, logits), stats = new_empty({r.rows, 2}, at::kFloat, logits);
+  auto wide = new_empty({r.rows + seqs}, at::kDouble, logits);
   RowArgs a = {};
   a.targets = t.const_data_ptr<int64_t>();
   a.mask = m.defined() ? m.const_data_ptr<bool>() : nullptr;
@@ -725,7 +722,7 @@ at::Tensor token_logprobs_bwd_ready(const at::Tensor& coef, const OptTensor& sca
   // A captured pass may be replayed with another scale, and then finds what the last one left: it computes all of it.
   const bool use_ready = ready.defined() && scale.has_value() &&
                          c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None;
-  auto grad = use_ready ? ready : at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
+  auto grad = use_ready ? ready : new_empty(logits.sizes(), logits.scalar_type(), logits);
   if (r.rows == 0) return grad;
   const auto t = targets.contiguous(), cf = coef.contiguous();
   const auto m = mask.has_value() ? mask->contiguous() : at::Tensor();

@@ -399,8 +399,8 @@ std::tuple<at::Tensor, at::Tensor> qk_norm_rope_fwd(const at::Tensor& q, const a
                                                     const at::Tensor& sin, const OptTensor& positions, double eps) {
   check_heads(q, k, q_weight, k_weight, cos, sin, positions);
   const c10::cuda::CUDAGuard guard(q.device());
-  auto qo = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
-  auto ko = at::empty(k.sizes(), k.options().memory_format(at::MemoryFormat::Contiguous));
+  auto qo = new_empty(q.sizes(), q.scalar_type(), q);
+  auto ko = new_empty(k.sizes(), k.scalar_type(), k);
   if (q.numel() + k.numel() == 0) return {qo, ko};
   Kept t;
   const int hpg = heads_per_group(q, k);
@@ -431,10 +431,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_bwd(
                         dk_out.scalar_type() == k.scalar_type() && dq_out.device() == q.device() && dk_out.device() == q.device(),
                     "gradients of the heads' shapes, dtype and device expected");
   const c10::cuda::CUDAGuard guard(q.device());
-  auto dq = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
-  auto dk = at::empty(k.sizes(), k.options().memory_format(at::MemoryFormat::Contiguous));
+  auto dq = new_empty(q.sizes(), q.scalar_type(), q);
+  auto dk = new_empty(k.sizes(), k.scalar_type(), k);
   const auto wsize = weight_grads ? q.size(3) : 0;
-  auto dwq = at::empty({wsize}, q_weight.options()), dwk = at::empty({wsize}, k_weight.options());
+  auto dwq = new_empty({wsize}, q_weight.scalar_type(), q), dwk = new_empty({wsize}, k_weight.scalar_type(), q);
   if (q.numel() + k.numel() == 0) return {dq, dk, dwq.zero_(), dwk.zero_()};
   Kept t;
   t.dq = rows16(dq_out);
@@ -457,7 +457,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_bwd(
   const int ctas = (int)std::min<int64_t>((units + groups - 1) / groups, resident);
   at::Tensor partial;
   if (weight_grads) {
-    partial = at::empty({ctas, 2, q.size(3)}, q.options().dtype(at::kFloat));
+    partial = new_empty({ctas, 2, q.size(3)}, at::kFloat, q);
     a.partial = partial.mutable_data_ptr<float>();
   }
   with_types(q, q_weight, [&](auto* tt, auto* tw, auto lanes) {

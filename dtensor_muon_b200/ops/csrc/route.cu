@@ -682,11 +682,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> route_fwd
   const c10::cuda::CUDAGuard guard(logits.device());
   const auto x = logits.stride(1) == 1 || logits.size(1) == 1 ? logits : logits.contiguous();
   const auto m = mask.has_value() ? mask->contiguous() : at::Tensor();
-  const auto f32 = logits.options().dtype(at::kFloat), i64 = logits.options().dtype(at::kLong);
   const int64_t t = x.size(0), e = x.size(1);
-  auto gates = at::empty({t, top_k}, logits.options().memory_format(at::MemoryFormat::Contiguous));
-  auto chosen = at::empty({t, top_k}, i64), counts = at::empty({e}, i64);
-  auto balance = at::empty({}, f32), z = at::empty({}, f32);
+  auto gates = new_empty({t, top_k}, logits.scalar_type(), logits);
+  auto chosen = new_empty({t, top_k}, at::kLong, logits), counts = new_empty({e}, at::kLong, logits);
+  auto balance = new_empty({}, at::kFloat, logits), z = new_empty({}, at::kFloat, logits);
   if (t == 0) return {gates, chosen, counts.zero_(), balance.zero_(), z.zero_()};
   Args a = args_of(x, m, top_k);
   a.gates = gates.mutable_data_ptr();
@@ -700,7 +699,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> route_fwd
     const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
     const int ctas = (int)std::min<int64_t>((t + groups - 1) / groups, (int64_t)sms * 4);
     // one workspace: the CTAs' parts, the totals and the ticket
-    auto work = at::empty({(e + 1) * (2 * (int64_t)ctas + 3) + 2}, f32);
+    auto work = new_empty({(e + 1) * (2 * (int64_t)ctas + 3) + 2}, at::kFloat, logits);
     a.total_p = reinterpret_cast<double*>(work.template mutable_data_ptr<float>());
     a.total_c = reinterpret_cast<int*>(a.total_p + e + 1);
     a.ticket = reinterpret_cast<unsigned*>(a.total_c + e + 1);
@@ -735,7 +734,7 @@ at::Tensor route_bwd(const OptTensor& dgates, const OptTensor& dbalance, const O
       TORCH_CHECK_VALUE((*s)->numel() == 1 && (*s)->scalar_type() == at::kFloat && (*s)->device() == logits.device(),
                         "dbalance, dz: one float32 value expected");
   const c10::cuda::CUDAGuard guard(logits.device());
-  auto out = at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
+  auto out = new_empty(logits.sizes(), logits.scalar_type(), logits);
   if (logits.size(0) == 0) return out;
   const auto x = logits.stride(1) == 1 || logits.size(1) == 1 ? logits : logits.contiguous();
   const auto m = mask.has_value() ? mask->contiguous() : at::Tensor();

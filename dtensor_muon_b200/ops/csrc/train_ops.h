@@ -3,6 +3,7 @@
 #pragma once
 
 #include <ATen/core/Tensor.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/util/Optional.h>
 
 #include <tuple>
@@ -10,6 +11,12 @@
 namespace dmb {
 
 using OptTensor = c10::optional<at::Tensor>;
+
+// A contiguous tensor on `like`'s device, without the way through the dispatcher: of a small call's host time each
+// allocation is a good part.
+inline at::Tensor new_empty(at::IntArrayRef sizes, at::ScalarType dtype, const at::Tensor& like) {
+  return at::detail::empty_cuda(sizes, dtype, like.device(), c10::nullopt);
+}
 
 int* device_error_word(int dev);
 void count_launches(int64_t n);  // kernels launched by these operators, for ops/_ext.py's counter
