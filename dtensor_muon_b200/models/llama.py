@@ -31,6 +31,7 @@ class LlamaConfig:
     rope_theta: float = 500000.0
     max_seq_len: int = 4096
     init_std: float = 0.02
+    qk_norm: bool = False  # RMS norm of every query and key head, in one pass with the rotation
 
     @property
     def head_dim(self) -> int:
@@ -85,6 +86,8 @@ class Attention(nn.Module):
         self.wk = nn.Linear(cfg.dim, cfg.n_kv_heads * cfg.head_dim, bias=False)
         self.wv = nn.Linear(cfg.dim, cfg.n_kv_heads * cfg.head_dim, bias=False)
         self.wo = nn.Linear(cfg.n_heads * cfg.head_dim, cfg.dim, bias=False)
+        self.q_norm = RMSNorm(cfg.head_dim, cfg.norm_eps) if cfg.qk_norm else None
+        self.k_norm = RMSNorm(cfg.head_dim, cfg.norm_eps) if cfg.qk_norm else None
         # set by train.build_llama(fused_gather=True): q/k/v through the fused
         # parameter all-gather + GEMM kernel (parallel.ag_gemm.GatherLinear)
         self.gather = None
@@ -98,7 +101,10 @@ class Attention(nn.Module):
             q = self.wq(x).view(B, S, -1, self.head_dim)
             k = self.wk(x).view(B, S, -1, self.head_dim)
             v = self.wv(x).view(B, S, -1, self.head_dim)
-        q, k = apply_rope(q, cos, sin), apply_rope(k, cos, sin)
+        if self.q_norm is not None:
+            q, k = _model_ops.qk_norm_rope(q, k, self.q_norm.weight, self.k_norm.weight, cos, sin, self.q_norm.eps)
+        else:
+            q, k = apply_rope(q, cos, sin), apply_rope(k, cos, sin)
         q, k, v = (t.transpose(1, 2) for t in (q, k, v))
         o = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=self.n_kv_heads != self.n_heads)
         o = o.transpose(1, 2).reshape(B, S, -1)

@@ -24,6 +24,8 @@ from .llama import Block, Llama, LlamaConfig
 class MixtralConfig(LlamaConfig):
     n_experts: int = 8
     top_k: int = 2
+    balance_coef: float = 0.0  # of the balance loss, summed over the layers
+    z_coef: float = 0.0  # of the mean squared log-sum-exp of the router logits
 
 
 MIXTRAL_PRESETS = {
@@ -68,6 +70,8 @@ class MoEFeedForward(nn.Module):
         self.w3 = nn.Parameter(torch.empty(cfg.n_experts, cfg.ffn_dim, cfg.dim))  # up
         self.w2 = nn.Parameter(torch.empty(cfg.n_experts, cfg.dim, cfg.ffn_dim))  # down
         self.ep = ep  # ExpertParallel or None (all experts local)
+        self.balance_coef, self.z_coef = cfg.balance_coef, cfg.z_coef
+        self.aux = None  # the last forward's router losses, where a coefficient asks for them
 
     def route(self, x: Tensor) -> tuple[Tensor, Tensor]:
         logits = self.router(x)
@@ -77,12 +81,19 @@ class MoEFeedForward(nn.Module):
     def forward(self, x: Tensor) -> Tensor:
         B, S, D = x.shape
         flat = x.reshape(-1, D)
-        idx, gates = self.route(flat)
+        counts = None
+        if self.balance_coef or self.z_coef:
+            gates, idx, counts, balance, z = _model_ops.route(self.router(flat), self.top_k)
+            gates = gates.to(x.dtype)
+            self.aux = self.balance_coef * balance + self.z_coef * z
+        else:
+            idx, gates = self.route(flat)
         w1, w3, w2 = (w.to_local() if hasattr(w, "to_local") else w for w in (self.w1, self.w3, self.w2))
         if self.ep is None:
             expert = idx.reshape(-1)
             order = torch.argsort(expert, stable=True)
-            counts = torch.bincount(expert, minlength=self.n_experts)
+            if counts is None:
+                counts = torch.bincount(expert, minlength=self.n_experts)
             rows = flat.repeat_interleave(self.top_k, dim=0)[order]
             y = expert_ffn(rows, counts, w1, w3, w2)
             out = torch.empty_like(y)
@@ -98,6 +109,11 @@ class Mixtral(Llama):
 
     def __init__(self, cfg: MixtralConfig, ep=None):
         super().__init__(cfg, block_factory=lambda: Block(cfg, ffn=MoEFeedForward(cfg, ep)))
+
+    def aux_loss(self) -> Tensor | None:
+        """Router losses of the last forward, over this rank's tokens; None without ``balance_coef`` and ``z_coef``."""
+        aux = [m.aux for m in self.modules() if isinstance(m, MoEFeedForward) and m.aux is not None]
+        return torch.stack(aux).sum() if aux else None
 
 
 __all__ = ["MIXTRAL_PRESETS", "MixtralConfig", "Mixtral", "MoEFeedForward", "expert_ffn", "mixtral_preset"]

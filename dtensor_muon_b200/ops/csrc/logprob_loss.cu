@@ -536,10 +536,9 @@ Rows rows_of(const at::Tensor& logits, const at::Tensor& targets, const OptTenso
   return r;
 }
 
-at::Tensor row_values(const at::Tensor& v, const at::Tensor& targets, const char* name) {
+void check_values(const at::Tensor& v, const at::Tensor& targets, const char* name) {
   TORCH_CHECK_VALUE(v.scalar_type() == at::kFloat && v.device() == targets.device() && v.sizes() == targets.sizes(), name,
                     ": float32 tensor of the targets' shape on their device expected");
-  return v.contiguous();
 }
 
 // Rows up to this length go to a warp each: 8 vectors per lane. (A CTA's 256 threads would have one each.)
@@ -624,10 +623,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
   TORCH_CHECK_VALUE(clip_low >= 0 && clip_low <= 1 && clip_high >= 0, "clip_low in [0, 1] and clip_high >= 0 expected, got ",
                     clip_low, " and ", clip_high);
   TORCH_CHECK_VALUE(kl_coef == 0 || ref_logp.has_value(), "kl_coef needs ref_logp");
+  check_values(old_logp, targets, "old_logp");
+  check_values(advantages, targets, "advantages");
+  if (ref_logp.has_value()) check_values(*ref_logp, targets, "ref_logp");
   const c10::cuda::CUDAGuard guard(logits.device());
-  const auto t = targets.contiguous(), old = row_values(old_logp, targets, "old_logp"),
-             adv = row_values(advantages, targets, "advantages");
-  const auto ref = ref_logp.has_value() ? row_values(*ref_logp, targets, "ref_logp") : at::Tensor();
+  const auto t = targets.contiguous(), old = old_logp.contiguous(), adv = advantages.contiguous();
+  const auto ref = ref_logp.has_value() ? ref_logp->contiguous() : at::Tensor();
   const auto m = mask.has_value() ? mask->contiguous() : at::Tensor();
   auto loss = new_empty({}, at::kFloat, logits), kl = new_empty({}, at::kFloat, logits), clipped = new_empty({}, at::kFloat, logits);
   auto logp = new_empty(targets.sizes(), at::kFloat, logits), coef = new_empty(targets.sizes(), at::kFloat, logits), stats = new_empty({r.rows, 2}, at::kFloat, logits);
@@ -676,8 +677,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> preferenc
                     "targets: [2 * pairs, seq] expected, the chosen sequences in front of the rejected ones");
   TORCH_CHECK_VALUE(beta > 0 && label_smoothing >= 0 && label_smoothing < 0.5,
                     "beta > 0 and label_smoothing in [0, 0.5) expected, got ", beta, " and ", label_smoothing);
+  check_values(ref_logp, targets, "ref_logp");
   const c10::cuda::CUDAGuard guard(logits.device());
-  const auto t = targets.contiguous(), ref = row_values(ref_logp, targets, "ref_logp");
+  const auto t = targets.contiguous(), ref = ref_logp.contiguous();
   const auto m = mask.has_value() ? mask->contiguous() : at::Tensor();
   const int seqs = (int)targets.size(0), seq = (int)targets.size(1);
   auto loss = new_empty({}, at::kFloat, logits), rewards = new_empty({seqs}, at::kFloat, logits), coef = new_empty({seqs}, at::kFloat, logits);

@@ -7,6 +7,10 @@ This is the public entry point a user calls to train with the framework:
     opt = build_optimizer(model)
     trainer = Trainer(model, opt)
     loss = trainer.step(tokens, targets)
+
+``Trainer.policy_step`` and ``Trainer.preference_step`` train on sampled answers
+or on pairs of answers instead, with the log-probabilities that
+``Trainer.score`` gave of an earlier or a frozen model.
 """
 
 from __future__ import annotations
@@ -16,6 +20,8 @@ import torch.distributed as dist
 from torch import Tensor, nn
 
 from .models.llama import Llama, LlamaConfig, lm_loss, muon_and_adam_params
+from .ops import model_ops
+from .ops.model_ops import PolicyLoss, PreferenceLoss
 from .optim import Muon
 
 
@@ -129,19 +135,56 @@ def synthetic_batch(batch: int, seq: int, vocab: int, generator: torch.Generator
 
 
 class Trainer:
-    """forward -> loss -> backward -> optimizer.step -> zero_grad."""
+    """forward -> loss -> backward -> optimizer.step -> zero_grad.
+
+    Every kind of step adds the model's ``aux_loss()`` (the router losses of a
+    sparse model that asks for them) to what it differentiates, and returns the
+    objective without it.
+    """
 
     def __init__(self, model: nn.Module, optimizer: torch.optim.Optimizer):
         self.model = model
         self.optimizer = optimizer
 
+    def _backward(self, loss: Tensor) -> None:
+        aux = self.model.aux_loss() if hasattr(self.model, "aux_loss") else None
+        (loss if aux is None else loss + aux).backward()
+
+    def _update(self) -> None:
+        self.optimizer.step()
+        self.optimizer.zero_grad(set_to_none=True)
+
     def forward_backward(self, tokens: Tensor, targets: Tensor) -> Tensor:
         loss = lm_loss(self.model(tokens), targets)
-        loss.backward()
+        self._backward(loss)
         return loss.detach()
 
     def step(self, tokens: Tensor, targets: Tensor) -> Tensor:
         loss = self.forward_backward(tokens, targets)
-        self.optimizer.step()
-        self.optimizer.zero_grad(set_to_none=True)
+        self._update()
         return loss
+
+    @torch.no_grad()
+    def score(self, tokens: Tensor, targets: Tensor, mask: Tensor | None = None) -> Tensor:
+        """fp32 log-probabilities of ``targets`` [B, S] under the model as it is; 0 where ``mask`` is false."""
+        return model_ops.token_logprobs(self.model(tokens), targets, mask=mask)
+
+    def policy_step(self, tokens: Tensor, targets: Tensor, old_logp: Tensor, advantages: Tensor,
+                    ref_logp: Tensor | None = None, mask: Tensor | None = None, clip_low: float = 0.2,
+                    clip_high: float = 0.2, kl_coef: float = 0.0) -> PolicyLoss:
+        """One clipped policy step on sampled tokens; arguments as :func:`ops.model_ops.policy_loss`."""
+        out = model_ops.policy_loss(self.model(tokens), targets, old_logp, advantages, ref_logp=ref_logp, mask=mask,
+                                    clip_low=clip_low, clip_high=clip_high, kl_coef=kl_coef)
+        self._backward(out.loss)
+        self._update()
+        return out._replace(loss=out.loss.detach())
+
+    def preference_step(self, tokens: Tensor, targets: Tensor, ref_logp: Tensor, mask: Tensor | None = None,
+                        beta: float = 0.1, label_smoothing: float = 0.0) -> PreferenceLoss:
+        """One step on pairs of answers, the chosen ones in front of the rejected ones; arguments as
+        :func:`ops.model_ops.preference_loss`."""
+        out = model_ops.preference_loss(self.model(tokens), targets, ref_logp, mask=mask, beta=beta,
+                                        label_smoothing=label_smoothing)
+        self._backward(out.loss)
+        self._update()
+        return out._replace(loss=out.loss.detach())

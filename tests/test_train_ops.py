@@ -6,7 +6,7 @@ import torch
 import train_ops_reference as ref
 
 from dtensor_muon_b200.models.llama import rope_tables
-from dtensor_muon_b200.ops import model_ops
+from dtensor_muon_b200.ops import _ext, model_ops
 
 DTYPES = [torch.float32, torch.bfloat16, torch.float16]
 
@@ -210,6 +210,26 @@ def refusals():
 def test_refusals(name, call):
     with pytest.raises(ValueError):
         call("cpu")
+
+
+@pytest.mark.skipif(not _ext.available(), reason="needs the built extension")
+@pytest.mark.parametrize("name,call", refusals(), ids=lambda v: v if isinstance(v, str) else "")
+def test_kernels_refuse_before_they_touch_a_device(name, call, monkeypatch):
+    """The CUDA kernels' own checks, seen without a GPU: on tensors that only say that they are on one."""
+    from types import SimpleNamespace
+
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    cuda = torch._C.DispatchKeySet(torch._C.DispatchKey.CUDA)
+
+    class Kernels:
+        def __getattr__(self, op):
+            return lambda *a: getattr(torch.ops.dmb, op).default.redispatch(cuda, *a)
+
+    monkeypatch.setattr(model_ops, "torch", SimpleNamespace(ops=SimpleNamespace(dmb=Kernels())))
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        with pytest.raises(ValueError):
+            call("cuda")
 
 
 def test_indices_outside_their_tables_are_refused():
