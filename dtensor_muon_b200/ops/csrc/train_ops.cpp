@@ -2,6 +2,7 @@
 // gradients as autograd functions in C++ (a Python formula would cost more host time than the
 // small calls take). The schemas, the CPU and the fake kernels are in ops/library.py. Each
 // autograd function calls its operators through the dispatcher, so that tracers see them.
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
@@ -176,7 +177,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> policy_loss_autograd(
     const Tensor& logits, const Tensor& targets, const Tensor& old_logp, const Tensor& advantages, const OptTensor& ref_logp,
     const OptTensor& mask, double clip_low, double clip_high, double kl_coef) {
   const auto keys = logits.key_set();
-  const bool plain = !keys.has(c10::DispatchKey::Python) && !keys.has(c10::DispatchKey::Functionalize);
+  const bool plain = !keys.has(c10::DispatchKey::Python) && !keys.has(c10::DispatchKey::Functionalize) &&
+                     !c10::impl::TorchDispatchModeTLS::any_modes_set();
   const bool grad_now = plain && at::GradMode::is_enabled() && logits.requires_grad() &&
                         c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None;
   auto r = PolicyLoss::apply(logits, targets, old_logp, advantages, ref_logp, mask, clip_low, clip_high, kl_coef, grad_now);

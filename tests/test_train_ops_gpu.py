@@ -349,6 +349,8 @@ def test_bad_targets_are_reported():
             assert torch.isnan(logp[1, 1]) and torch.equal(logp[keep], good[keep])
             with pytest.raises(RuntimeError, match="error code 3"):
                 _ext.check_device_errors("cuda")
+            (g,) = torch.autograd.grad(logp, x, torch.ones_like(logp))
+            assert torch.isnan(g[1, 1]).all() and not torch.isnan(g[keep]).any()
             p = model_ops.policy_loss(x, t, old, adv)
             assert torch.isnan(p.loss)
             (g,) = torch.autograd.grad(p.loss, x)
@@ -378,6 +380,110 @@ def test_backward_twice_scaled_and_refused_twice():
         x.mul_(2)
     with pytest.raises(RuntimeError, match="inplace"):
         p.loss.backward()
+
+
+def test_policy_gradient_under_modes_hooks_and_accumulation():
+    from torch.utils._python_dispatch import TorchDispatchMode
+    from torch.utils.checkpoint import checkpoint
+
+    logits, targets, mask, old, adv, frozen = _tokens(2, 40, 5000, BF16)
+
+    def loss(x):
+        return model_ops.policy_loss(x, targets, old, adv, ref_logp=frozen, mask=mask, kl_coef=0.1).loss
+
+    x = logits.detach().requires_grad_()
+    (want,) = torch.autograd.grad(loss(x), x)
+    seen = []
+
+    class Mode(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    with Mode():
+        out = loss(x)
+        (got,) = torch.autograd.grad(out, x)
+    assert torch.equal(got, want)
+    assert any("policy_loss" in f for f in seen) and any("token_logprobs_backward" in f for f in seen)
+    (got,) = torch.autograd.grad(checkpoint(loss, x, use_reentrant=False), x)
+    assert torch.equal(got, want)
+    with torch.autograd.graph.save_on_cpu():
+        out = loss(x)
+    assert torch.equal(torch.autograd.grad(out, x)[0], want)
+    x.grad = None
+    loss(x).backward()
+    loss(x).backward()
+    ref.check(dict(grad=x.grad), dict(grad=(2 * want.double(), want.double().abs() * 2**-7)))
+    # a scaled loss, as in gradient accumulation
+    x.grad = None
+    (loss(x) / 4).backward()
+    ref.check(dict(grad=x.grad), ref.policy_loss(logits, targets, old, adv, frozen, mask, kl_coef=0.1, scale=0.25))
+
+
+def test_long_rows():
+    for dtype in (BF16, FP32):
+        _check_losses(*_tokens(2, 2, 300001, dtype))
+
+
+# ---------------------------------------------------------- offsets past 32 bits
+
+
+def test_losses_of_more_than_2_31_logits():
+    rows, v = 17000, 128256
+    logits = torch.zeros(rows, v, device="cuda", dtype=BF16)
+    few = _tokens(1, 3, v, BF16)
+    logits[-3:] = few[0][0]
+    targets = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    targets[-3:] = few[1][0]
+    mask = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    mask[-3:] = True
+    x = logits.requires_grad_()
+    old, adv = torch.zeros(rows, device="cuda"), torch.zeros(rows, device="cuda")
+    old[-3:], adv[-3:] = few[3][0], few[4][0]
+    want = ref.policy_loss(few[0][0], few[1][0], few[3][0], few[4][0])
+    p = model_ops.policy_loss(x, targets, old, adv, mask=mask)
+    (g,) = torch.autograd.grad(p.loss, x)
+    ref.check(dict(loss=p.loss, logp=p.logp[-3:], grad=g[-3:]), want)
+    assert not g[:-3:1000].any()
+    del g
+    logp = model_ops.token_logprobs(x, targets, mask=mask)
+    (g,) = torch.autograd.grad(logp, x, torch.ones_like(logp))
+    ref.check(dict(logp=logp[-3:], grad=g[-3:]), ref.token_logprobs(few[0][0], few[1][0], None, torch.ones(3, device="cuda")))
+
+
+def test_heads_of_more_than_2_31_values():
+    tokens, h, d = 70000, 256, 128
+    q = torch.zeros(1, tokens, h, d, device="cuda", dtype=BF16)
+    few = _qk(1, 2, h, 1, d, BF16)
+    q[:, -2:] = few[0]
+    k = torch.zeros(1, tokens, 1, d, device="cuda", dtype=BF16)
+    pos = torch.zeros(1, tokens, dtype=torch.int32, device="cuda")
+    pos[0, -1] = 5
+    x = q.requires_grad_()
+    y, _ = model_ops.qk_norm_rope(x, k, few[2], few[3], few[4], few[5], positions=pos)
+    one = torch.ones((), device="cuda", dtype=BF16)
+    (g,) = torch.autograd.grad(y, x, one.expand_as(y))
+    want = ref.qk_norm_rope(few[0], k[:, -2:], few[2], few[3], few[4], few[5], 1e-5, pos[:, -2:],
+                            one.expand(1, 2, h, d), k[:, -2:])
+    ref.check(dict(q=y[:, -2:], dq=g[:, -2:]), want)
+
+
+def test_route_of_more_than_2_31_logits():
+    tokens, e = 4_200_000, 512
+    x = torch.zeros(tokens, e, device="cuda", dtype=BF16)
+    few = _randn(3, e, g=_gen(1), dtype=BF16)
+    x[-3:] = few
+    mask = torch.zeros(tokens, dtype=torch.bool, device="cuda")
+    mask[-3:] = True
+    x.requires_grad_()
+    r = model_ops.route(x, 2, mask=mask)
+    dg = _randn(3, 2, g=_gen(2), dtype=BF16)
+    wide = torch.zeros(tokens, 2, device="cuda", dtype=BF16)
+    wide[-3:] = dg
+    (g,) = torch.autograd.grad([r.gates, r.balance], x, [wide, torch.ones((), device="cuda")])
+    want = ref.route(few, 2, None, dg, 1.0)
+    ref.check(dict(gates=r.gates[-3:], experts=r.experts[-3:], counts=r.counts, balance=r.balance, z=r.z, grad=g[-3:]), want)
+    assert not g[: -3 : 10007].any()
 
 
 # ------------------------------------------------------------------ everywhere
