@@ -8,12 +8,22 @@
 //   gradient of any of them: dx_j = c_t ([j == y] - softmax(x)_j), c_t = dL / dlogp_t
 //
 // One pass over the logits forward (running maximum m and sum s per thread, joined over the
-// row), one read and one write backward. The statistics kept between the two are (m, s) and not
-// the log-sum-exp: exp(x - m) / s has no large terms that cancel, so its relative error does not
-// grow with the size of the logits. What follows from a row's logp (ratio, KL estimate, their
-// derivatives) is computed in 64 bits by the one thread that joins the row, from x_y - m and s:
-// differences of log-probabilities nearly cancel, and rounding them first would be what is lost.
-// Rows that do not count are not read.
+// row), one read and one write backward; policy_loss, whose coefficients hang on their own row
+// only, writes the gradient with the loss and reads the logits once. The statistics kept between
+// the two are (m, s) and not the log-sum-exp: exp(x - m) / s has no large terms that cancel, so
+// its relative error does not grow with the size of the logits. What follows from a row's logp
+// (ratio, KL estimate, their derivatives) is computed in 64 bits by the one thread that joins the
+// row, from x_y - m and s: differences of log-probabilities nearly cancel, and rounding them first
+// would be what is lost. Rows that do not count are not read.
+//
+// Bound by memory, with the exponentials (16 a cycle and SM) close behind: arithmetic is packed,
+// two fp32 values to an instruction. Measured on one B200, alone on the device (6.45 TB/s copied):
+//   scoring 4096 rows of 32000 bf16        48 us, 5.5 TB/s (262 MB)
+//   policy loss and gradient, 4096 rows of 128256 bf16, a quarter masked
+//                                         363 us, 5.1 TB/s (1.84 GB; two passes took 448)
+//   preference loss and gradient, 4096 rows of 32000 bf16, 40 % masked
+//                                         108 us, 5.3 TB/s (577 MB: the logits are read twice, as
+//                                         a coefficient hangs on the sums of both sequences)
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
@@ -163,18 +173,23 @@ __device__ __forceinline__ void scan_vectors(const Raw8<T> (&raw)[kUnroll], floa
   s += x.x + x.y;
 }
 
-// Calls use(raw, base) for the vectors [v0, v1) of p, of which thread `tid` of `nt` takes every nt-th: kUnroll of them at a
-// time, at base, base + nt ... (-inf beyond v1).
-template <typename T, typename F>
-__device__ __forceinline__ void stream_row(const T* p, int v0, int v1, int tid, int nt, F&& use) {
+// kUnroll of a thread's vectors: at base, base + nt ..., -inf from v1 on.
+template <typename T>
+__device__ __forceinline__ void load_group(Raw8<T> (&raw)[kUnroll], const T* p, int base, int v1, int nt) {
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const int v = base + u * nt;
+    raw[u] = v < v1 ? load_raw8<T>(p + (long long)v * 8) : raw_neg_inf<T>();
+  }
+}
+
+// Adds the vectors [v0, v1) of p, of which thread `tid` of `nt` takes every nt-th, to its maximum and sum.
+template <typename T>
+__device__ __forceinline__ void scan_row(const T* p, int v0, int v1, int tid, int nt, float& m, float& s) {
   for (int base = v0 + tid; base < v1; base += nt * kUnroll) {
     Raw8<T> raw[kUnroll];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int v = base + u * nt;
-      raw[u] = v < v1 ? load_raw8<T>(p + (long long)v * 8) : raw_neg_inf<T>();
-    }
-    use(raw, base);
+    load_group<T>(raw, p, base, v1, nt);
+    scan_vectors<T>(raw, m, s);
   }
 }
 
@@ -256,7 +271,7 @@ __global__ void __launch_bounds__(32 * kWarpRows) warp_row_kernel(const RowArgs 
   const float xy = lane == 0 ? target_logit(a, p, a.targets[row]) : 0.f;
   const int vecs = (a.vocab - head) / 8;
   float m = -INFINITY, s = 0.f;
-  stream_row<T>(p + head, 0, vecs, lane, 32, [&](const Raw8<T>(&raw)[kUnroll], int) { scan_vectors<T>(raw, m, s); });
+  scan_row<T>(p + head, 0, vecs, lane, 32, m, s);
   scan_ends<T>(p, a.vocab, head, vecs, lane, 32, m, s);
   warp_join(m, s);
   if (lane == 0) finish_row<MODE>(a, row, xy, m, s);
@@ -306,29 +321,38 @@ __device__ __forceinline__ void fill_zero(T* g, int n, int share, int shares, in
     for (int j = tid; j < head + (n - tail); j += nt) g[j < head ? j : tail + j - head] = from_float<T>(0.f);
 }
 
-// Gradient of the vectors [v0, v1) of p.
+// Gradient of the vectors [v0, v1) of p; `raw` holds the thread's first ones.
 template <typename T>
-__device__ __forceinline__ void grad_row(const T* p, T* g, int v0, int v1, int tid, int nt, float m, float neg, int hot, float c) {
+__device__ __forceinline__ void grad_row(Raw8<T> (&raw)[kUnroll], const T* p, T* g, int v0, int v1, int tid, int nt, float m,
+                                         float neg, int hot, float c) {
   const bool aligned = (reinterpret_cast<uintptr_t>(g) & 15) == 0;
-  stream_row<T>(p, v0, v1, tid, nt, [&](const Raw8<T>(&raw)[kUnroll], int base) {
+  int base = v0 + tid;
+  auto write = [&] {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const int v = base + u * nt;
       if (v < v1) grad_vector<T>(raw[u], g + (long long)v * 8, aligned, m, neg, hot - v * 8, c);
     }
-  });
+  };
+  write();
+  for (base += nt * kUnroll; base < v1; base += nt * kUnroll) {
+    load_group<T>(raw, p, base, v1, nt);
+    write();
+  }
 }
 
 constexpr int kRowThreads = 256;
 // With GRAD a row is split until a part is no longer than this: fewer rows at once, which are still in the L2 when the
-// gradient is written. 128256 bf16 logits in four parts take 380 us for 4096 rows, in two 395, in one 406 (each row then
-// comes from memory twice), and in eight, of which each has too little to do between the cluster's barriers, 421.
+// gradient is written. 4096 rows of 128256 bf16 logits, a quarter of them masked, took 380 us in four parts, 395 in two, 406
+// in one (each row then comes from memory twice), and 421 in eight, which have too little to do between two barriers.
 constexpr int kGradPart = 80 * 1024;
 
 // A cluster of CTAs per row, most often of one: with fewer rows than the GPU has room for a row is split, and the parts are
 // joined through the first CTA's shared memory. With GRAD the row's gradient follows at once, while the row is in the L2.
+// GRAD: registers for six CTAs to an SM (353 us for the rows above; four, which is what the compiler comes to, take 380, and
+// eight, which spill, 397), five for fp32. Without, six or seven come by themselves.
 template <typename T, Mode MODE, bool GRAD>
-__global__ void __launch_bounds__(kRowThreads) row_kernel(const RowArgs a) {
+__global__ void __launch_bounds__(kRowThreads, !GRAD ? 1 : sizeof(T) == 2 ? 6 : 5) row_kernel(const RowArgs a) {
   constexpr int NT = kRowThreads;
   __shared__ float2 warps[NT / 32];
   __shared__ float2 parts[8];  // of the cluster's CTAs, in the first one
@@ -347,10 +371,16 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const RowArgs a) {
   const T* p = row_of<T>(a.logits, a.stride_b, a.stride_s, a.seq, row);
   const int head = head_of(p, a.vocab), vecs = (a.vocab - head) / 8;
   const int each = (vecs + split - 1) / split, v0 = min(rank * each, vecs), v1 = min(v0 + each, vecs);
+  if (GRAD && tid == 0 && v1 > v0)  // the whole part to the L2, at once: 381 to 364 us. (Without GRAD 48 become 51.)
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p + head + (long long)v0 * 8),
+                 "r"((uint32_t)(v1 - v0) * 8 * (uint32_t)sizeof(T))
+                 : "memory");
   const int64_t y = a.targets[row];  // looked at once the row has been read
   float m = -INFINITY, s = 0.f;
-  stream_row<T>(p + head, v0, v1, tid, NT, [&](const Raw8<T>(&raw)[kUnroll], int) { scan_vectors<T>(raw, m, s); });
+  scan_row<T>(p + head, v0, v1, tid, NT, m, s);
   if (rank == 0) scan_ends<T>(p, a.vocab, head, vecs, tid, NT, m, s);
+  Raw8<T> first[kUnroll];  // of the second pass, on their way while the row is joined
+  if constexpr (GRAD) load_group<T>(first, p + head, v0 + tid, v1, NT);
   warp_join(m, s);
   if ((tid & 31) == 0) warps[tid >> 5] = make_float2(m, s);
   __syncthreads();
@@ -381,7 +411,7 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const RowArgs a) {
       return;
     }
     const int hot = y >= 0 && y < a.vocab ? (int)y - head : -8;
-    grad_row<T>(p + head, g + head, v0, v1, tid, NT, k.x, k.y, hot, k.z);
+    grad_row<T>(first, p + head, g + head, v0, v1, tid, NT, k.x, k.y, hot, k.z);
     if (rank == 0) grad_ends<T>(p, g, a.vocab, head, vecs, tid, NT, k.x, k.y, (int)y, k.z);
   }
 }
@@ -422,7 +452,9 @@ __global__ void __launch_bounds__(kGradThreads) logprob_grad_kernel(const GradAr
     const float2 st = a.stats[row];
     const int64_t y = a.targets[row];
     const int hot = y >= 0 && y < a.vocab ? (int)y - head : -8;
-    grad_row<T>(p + head, g + head, v0, v1, threadIdx.x, kGradThreads, st.x, -c / st.y, hot, c);
+    Raw8<T> raw[kUnroll];
+    load_group<T>(raw, p + head, v0 + threadIdx.x, v1, kGradThreads);
+    grad_row<T>(raw, p + head, g + head, v0, v1, threadIdx.x, kGradThreads, st.x, -c / st.y, hot, c);
     if (chunk == 0) grad_ends<T>(p, g, a.vocab, head, vecs, threadIdx.x, kGradThreads, st.x, -c / st.y, (int)y, c);
   }
 }
