@@ -18,11 +18,11 @@
 //
 // Bound by memory, with the exponentials (16 a cycle and SM) close behind: arithmetic is packed,
 // two fp32 values to an instruction. Measured on one B200, alone on the device (6.45 TB/s copied):
-//   scoring 4096 rows of 32000 bf16        48 us, 5.5 TB/s (262 MB)
+//   scoring 4096 rows of 32000 bf16        47 us, 5.6 TB/s (262 MB)
 //   policy loss and gradient, 4096 rows of 128256 bf16, a quarter masked
-//                                         363 us, 5.1 TB/s (1.84 GB; two passes took 448)
+//                                         358 us, 5.1 TB/s (1.84 GB; two passes took 448)
 //   preference loss and gradient, 4096 rows of 32000 bf16, 40 % masked
-//                                         108 us, 5.3 TB/s (577 MB: the logits are read twice, as
+//                                         107 us, 5.4 TB/s (577 MB: the logits are read twice, as
 //                                         a coefficient hangs on the sums of both sequences)
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
@@ -41,7 +41,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLog2eRest = (float)(1.4426950408889634 - (double)kLog2e);
+constexpr float kLog2eUp = 1.4426951408386230f;  // the next larger fp32
 constexpr int kUnroll = 4;         // 8-element vectors that a thread takes at once
 constexpr int kWarpRows = 4;       // rows of a CTA whose warps have one each
 
@@ -59,7 +59,7 @@ struct RowArgs {
   int* error;
   // policy and preference
   const float *old_logp, *advantages, *ref_logp;
-  float clip_low, clip_high, kl_coef;
+  double clip_low, clip_high, kl_coef;
   const int* count;  // rows that the mask keeps; null: all
   float *row_loss, *row_kl, *coef;
   bool* row_clipped;
@@ -156,18 +156,16 @@ __device__ __forceinline__ void scan_vectors(const Raw8<T> (&raw)[kUnroll], floa
   const float mx = fmaxf(m, max_of<T>(raw)), a = anchor(mx);
   if (mx != m) s *= expf(m - a);
   m = mx;
-  const F2 neg = f2(-a, -a), c = f2(kLog2e, kLog2e), rest = f2(kLog2eRest, kLog2eRest);
+  // log2 e in 32 bits is 1.3e-8 of itself too small, which shifts every log-probability to the same side by that times its
+  // distance from the mean logit; the next larger number is 6.9e-8 too large. One value in eight with that one leaves 3e-9.
+  const F2 neg = f2(-a, -a), c = f2(kLog2e, kLog2e), up = f2(kLog2e, kLog2eUp);
   F2 sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
     F2 v[4];
     unpack_f2<T>(raw[u], v);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const F2 t = v[k] + neg;
-      // what the constant loses in 32 bits is 1.3e-8 of the product, always to the same side: see finish_row
-      sum[k & 1] = sum[k & 1] + ex2(fma2(t, c, t * rest));
-    }
+    for (int k = 0; k < 4; ++k) sum[k & 1] = sum[k & 1] + ex2((v[k] + neg) * (k == 3 ? up : c));
   }
   const float2 x = f2_values(sum[0] + sum[1]);
   s += x.x + x.y;
@@ -219,9 +217,9 @@ __device__ __forceinline__ float finish_row(const RowArgs& a, int row, float xy,
     if (a.ref_logp) {
       const double d = (double)a.ref_logp[row] - lp, e = expm1(d);
       kl = e - d;
-      if (a.kl_coef != 0.f) {
-        loss += (double)a.kl_coef * kl;
-        coef -= (double)a.kl_coef * e;
+      if (a.kl_coef != 0) {
+        loss += a.kl_coef * kl;
+        coef -= a.kl_coef * e;
       }
     }
     a.row_loss[row] = (float)loss;
@@ -349,10 +347,10 @@ constexpr int kGradPart = 80 * 1024;
 
 // A cluster of CTAs per row, most often of one: with fewer rows than the GPU has room for a row is split, and the parts are
 // joined through the first CTA's shared memory. With GRAD the row's gradient follows at once, while the row is in the L2.
-// GRAD: registers for six CTAs to an SM (353 us for the rows above; four, which is what the compiler comes to, take 380, and
-// eight, which spill, 397), five for fp32. Without, six or seven come by themselves.
+// Registers for six CTAs to an SM, five for fp32, which the compiler does not come to by itself. With GRAD the rows above
+// take 350 us so, 380 with four and 397 with eight (which spill); 4096 rows of 32000 take 47 us without GRAD, 54 with four.
 template <typename T, Mode MODE, bool GRAD>
-__global__ void __launch_bounds__(kRowThreads, !GRAD ? 1 : sizeof(T) == 2 ? 6 : 5) row_kernel(const RowArgs a) {
+__global__ void __launch_bounds__(kRowThreads, sizeof(T) == 2 ? 6 : 5) row_kernel(const RowArgs a) {
   constexpr int NT = kRowThreads;
   __shared__ float2 warps[NT / 32];
   __shared__ float2 parts[8];  // of the cluster's CTAs, in the first one
@@ -505,8 +503,8 @@ __global__ void __launch_bounds__(kReduceThreads) policy_reduce_kernel(const Row
 }
 
 // A warp sums each sequence, then a thread takes each pair. coef[i] is the derivative by each of sequence i's logp.
-__global__ void __launch_bounds__(kReduceThreads) preference_reduce_kernel(const double* diff, int pairs, int seq, float beta,
-                                                                          float smoothing, double* sums, float* loss,
+__global__ void __launch_bounds__(kReduceThreads) preference_reduce_kernel(const double* diff, int pairs, int seq, double beta,
+                                                                          double smoothing, double* sums, float* loss,
                                                                           float* rewards, float* coef) {
   __shared__ double smem[32];
   const int lane = threadIdx.x & 31;
@@ -523,12 +521,12 @@ __global__ void __launch_bounds__(kReduceThreads) preference_reduce_kernel(const
   __syncthreads();
   double l = 0;
   for (int i = threadIdx.x; i < pairs; i += kReduceThreads) {
-    const double h = (double)beta * (sums[i] - sums[pairs + i]);
+    const double h = beta * (sums[i] - sums[pairs + i]);
     const double tail = log1p(exp(-fabs(h)));  // log sigmoid(h) = min(h, 0) - tail
     const double up = fmin(h, 0.0) - tail, down = fmin(-h, 0.0) - tail;
     l -= (1.0 - smoothing) * up + smoothing * down;
     const double sig = h >= 0 ? 1.0 / (1.0 + exp(-h)) : exp(h) / (1.0 + exp(h));
-    const double dh = (double)smoothing * sig - (1.0 - smoothing) * (1.0 - sig);
+    const double dh = smoothing * sig - (1.0 - smoothing) * (1.0 - sig);
     coef[i] = (float)(beta * dh / pairs);
     coef[pairs + i] = (float)(-beta * dh / pairs);
   }
@@ -676,9 +674,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
   a.old_logp = old.const_data_ptr<float>();
   a.advantages = adv.const_data_ptr<float>();
   a.ref_logp = ref.defined() ? ref.const_data_ptr<float>() : nullptr;
-  a.clip_low = (float)clip_low;
-  a.clip_high = (float)clip_high;
-  a.kl_coef = (float)kl_coef;
+  a.clip_low = clip_low;
+  a.clip_high = clip_high;
+  a.kl_coef = kl_coef;
   a.row_loss = work.mutable_data_ptr<float>();
   a.row_kl = a.row_loss + r.rows;
   int* count = reinterpret_cast<int*>(a.row_kl + r.rows);
@@ -728,7 +726,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> preferenc
   a.row_diff = wide.mutable_data_ptr<double>();
   const auto stream = at::cuda::getCurrentCUDAStream();
   launch_rows<kPreference>(r, a, stream);
-  preference_reduce_kernel<<<1, kReduceThreads, 0, stream>>>(a.row_diff, seqs / 2, seq, (float)beta, (float)label_smoothing,
+  preference_reduce_kernel<<<1, kReduceThreads, 0, stream>>>(a.row_diff, seqs / 2, seq, beta, label_smoothing,
                                                             a.row_diff + r.rows, loss.mutable_data_ptr<float>(),
                                                             rewards.mutable_data_ptr<float>(), coef.mutable_data_ptr<float>());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
