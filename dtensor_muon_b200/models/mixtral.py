@@ -73,6 +73,10 @@ class MoEFeedForward(nn.Module):
         self.balance_coef, self.z_coef = cfg.balance_coef, cfg.z_coef
         self.aux = None  # the last forward's router losses, where a coefficient asks for them
 
+    def __getstate__(self):
+        # a copy of the model takes none of the last forward's graph along
+        return dict(self.__dict__, aux=None)
+
     def route(self, x: Tensor) -> tuple[Tensor, Tensor]:
         logits = self.router(x)
         top, idx = torch.topk(logits, self.top_k, dim=-1)

@@ -255,26 +255,6 @@ __device__ __forceinline__ float target_logit(const RowArgs& a, const T* p, int6
   return to_float(p[y]);
 }
 
-// One warp per row, for short rows.
-template <typename T, Mode MODE>
-__global__ void __launch_bounds__(32 * kWarpRows) warp_row_kernel(const RowArgs a) {
-  const int row = blockIdx.x * kWarpRows + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= a.rows) return;
-  if (a.mask && !a.mask[row]) {
-    if (lane == 0) skip_row<MODE>(a, row);
-    return;
-  }
-  const T* p = row_of<T>(a.logits, a.stride_b, a.stride_s, a.seq, row);
-  const int head = head_of(p, a.vocab);
-  const float xy = lane == 0 ? target_logit(a, p, a.targets[row]) : 0.f;
-  const int vecs = (a.vocab - head) / 8;
-  float m = -INFINITY, s = 0.f;
-  scan_row<T>(p + head, 0, vecs, lane, 32, m, s);
-  scan_ends<T>(p, a.vocab, head, vecs, lane, 32, m, s);
-  warp_join(m, s);
-  if (lane == 0) finish_row<MODE>(a, row, xy, m, s);
-}
-
 // Gradient of one vector; `hot` is the target's place in it, if it has one in 0..7.
 template <typename T>
 __device__ __forceinline__ void grad_vector(const Raw8<T>& raw, T* to, bool aligned, float m, float neg, int hot, float c) {
@@ -336,6 +316,41 @@ __device__ __forceinline__ void grad_row(Raw8<T> (&raw)[kUnroll], const T* p, T*
   for (base += nt * kUnroll; base < v1; base += nt * kUnroll) {
     load_group<T>(raw, p, base, v1, nt);
     write();
+  }
+}
+
+// One warp per row, for short rows. With GRAD the row's gradient follows at once.
+template <typename T, Mode MODE, bool GRAD>
+__global__ void __launch_bounds__(32 * kWarpRows) warp_row_kernel(const RowArgs a) {
+  const int row = blockIdx.x * kWarpRows + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= a.rows) return;
+  T* g = GRAD ? static_cast<T*>(a.grad) + (long long)row * a.vocab : nullptr;
+  if (a.mask && !a.mask[row]) {
+    if (lane == 0) skip_row<MODE>(a, row);
+    if (GRAD) fill_zero<T>(g, a.vocab, 0, 1, lane, 32);
+    return;
+  }
+  const T* p = row_of<T>(a.logits, a.stride_b, a.stride_s, a.seq, row);
+  const int head = head_of(p, a.vocab), vecs = (a.vocab - head) / 8;
+  const int64_t y = a.targets[row];
+  const float xy = lane == 0 ? target_logit(a, p, y) : 0.f;
+  float m = -INFINITY, s = 0.f;
+  scan_row<T>(p + head, 0, vecs, lane, 32, m, s);
+  scan_ends<T>(p, a.vocab, head, vecs, lane, 32, m, s);
+  warp_join(m, s);
+  float c = 0.f;
+  if (lane == 0) c = finish_row<MODE>(a, row, xy, m, s);
+  if constexpr (GRAD) {
+    c = __shfl_sync(~0u, c, 0);
+    if (c == 0.f) {
+      fill_zero<T>(g, a.vocab, 0, 1, lane, 32);
+      return;
+    }
+    const int hot = y >= 0 && y < a.vocab ? (int)y - head : -8;
+    Raw8<T> raw[kUnroll];
+    load_group<T>(raw, p + head, lane, vecs, 32);
+    grad_row<T>(raw, p + head, g + head, 0, vecs, lane, 32, anchor(m), -c / s, hot, c);
+    grad_ends<T>(p, g, a.vocab, head, vecs, lane, 32, anchor(m), -c / s, (int)y, c);
   }
 }
 
@@ -430,30 +445,33 @@ struct GradArgs {
 
 constexpr int kGradThreads = 256;
 
-// dx_j = c ([j == y] - exp(x_j - m) / s). A CTA takes one of a row's `chunks` at a time. Rows with c = 0 are not read.
-template <typename T>
+// dx_j = c ([j == y] - exp(x_j - m) / s). A group of NT threads (a CTA, or a warp for short rows) takes one of a row's
+// `chunks` at a time. Rows with c = 0 are not read.
+template <typename T, int NT>
 __global__ void __launch_bounds__(kGradThreads) logprob_grad_kernel(const GradArgs a) {
   const float scale = a.scale ? *a.scale : 1.f;
   if (a.ready && scale == 1.f) return;
-  for (unsigned unit = blockIdx.x; unit < (unsigned)a.rows * a.chunks; unit += gridDim.x) {
+  constexpr unsigned kPer = kGradThreads / NT;
+  const int tid = threadIdx.x % NT;
+  for (unsigned unit = blockIdx.x * kPer + threadIdx.x / NT; unit < (unsigned)a.rows * a.chunks; unit += gridDim.x * kPer) {
     const int row = unit / (unsigned)a.chunks, chunk = unit - row * a.chunks;
     T* g = static_cast<T*>(a.grad) + (long long)row * a.vocab;
     float c = a.mask && !a.mask[row] ? 0.f : a.coef[(unsigned)row / (unsigned)a.rows_per_coef];
     if (c != 0.f) c *= scale;
     if (c == 0.f) {
-      fill_zero<T>(g, a.vocab, chunk, a.chunks, threadIdx.x, kGradThreads);
+      fill_zero<T>(g, a.vocab, chunk, a.chunks, tid, NT);
       continue;
     }
     const T* p = row_of<T>(a.logits, a.stride_b, a.stride_s, a.seq, row);
     const int head = head_of(p, a.vocab), vecs = (a.vocab - head) / 8;
-    const int each = ((unsigned)vecs + a.chunks - 1) / (unsigned)a.chunks, v0 = chunk * each, v1 = min(v0 + each, vecs);
+    const int each = ((unsigned)vecs + a.chunks - 1) / (unsigned)a.chunks, v0 = min(chunk * each, vecs), v1 = min(v0 + each, vecs);
+    Raw8<T> raw[kUnroll];
+    load_group<T>(raw, p + head, v0 + tid, v1, NT);
     const float2 st = a.stats[row];
     const int64_t y = a.targets[row];
     const int hot = y >= 0 && y < a.vocab ? (int)y - head : -8;
-    Raw8<T> raw[kUnroll];
-    load_group<T>(raw, p + head, v0 + threadIdx.x, v1, kGradThreads);
-    grad_row<T>(raw, p + head, g + head, v0, v1, threadIdx.x, kGradThreads, st.x, -c / st.y, hot, c);
-    if (chunk == 0) grad_ends<T>(p, g, a.vocab, head, vecs, threadIdx.x, kGradThreads, st.x, -c / st.y, (int)y, c);
+    grad_row<T>(raw, p + head, g + head, v0, v1, tid, NT, st.x, -c / st.y, hot, c);
+    if (chunk == 0) grad_ends<T>(p, g, a.vocab, head, vecs, tid, NT, st.x, -c / st.y, (int)y, c);
   }
 }
 
@@ -573,10 +591,12 @@ void check_values(const at::Tensor& v, const at::Tensor& targets, const char* na
                     ": float32 tensor of the targets' shape on their device expected");
 }
 
-// Rows up to this length go to a warp each: 8 vectors per lane. (A CTA's 256 threads would have one each.)
-constexpr int kWarpRowMax = 2048;
-
-bool in_warps(const Rows& r) { return r.vocab <= kWarpRowMax; }
+// Whether rows go to a warp each: where they are short and many. Warp and CTA, log-probabilities and gradients of bf16 rows:
+// 4096 of 1024 4.1 + 4.3 and 13 + 13 us, 16384 of 4096 33 + 40 and 62 + 63 us, 4096 of 8192 19 + 19 and 20 + 21 us; 74 of
+// 1024 2.6 + 2.9 and 2.8 + 2.4 us, 74 of 4096 3.9 + 5.2 and 2.9 + 2.5 us.
+bool in_warps(const Rows& r) {
+  return r.vocab <= 8192 && r.rows >= 8 * at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+}
 
 template <typename T, Mode MODE, bool GRAD>
 void launch_row_kernel(const RowArgs& a, int split, cudaStream_t stream) {
@@ -605,11 +625,17 @@ void launch_rows(const Rows& r, RowArgs& a, cudaStream_t stream) {
   with_element(r.logits.scalar_type(), [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     if (in_warps(r)) {
-      warp_row_kernel<T, MODE><<<(r.rows + kWarpRows - 1) / kWarpRows, 32 * kWarpRows, 0, stream>>>(a);
+      const unsigned grid = (r.rows + kWarpRows - 1) / kWarpRows;
+      bool done = false;
+      if constexpr (MODE == kPolicy) {
+        if ((done = a.grad != nullptr)) warp_row_kernel<T, MODE, true><<<grid, 32 * kWarpRows, 0, stream>>>(a);
+      }
+      if (!done) warp_row_kernel<T, MODE, false><<<grid, 32 * kWarpRows, 0, stream>>>(a);
       C10_CUDA_KERNEL_LAUNCH_CHECK();
       return;
     }
-    // Few rows: split each until every SM has two CTAs or a part is down to two rounds of its CTA's loads.
+    // Few rows: split each until every SM has two CTAs or a part is down to two rounds of its CTA's loads. (Rows of 128256
+    // bf16, split and whole: 4 of them 4.8 and 10 us, 64 7.1 and 13 us, 150 15 and 20 us.)
     const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
     int split = 1;
     while (split < 8 && (int64_t)r.rows * split < 2 * sms && r.vocab / split > 2 * kRowThreads * 8 * kUnroll) split *= 2;
@@ -689,7 +715,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
     C10_CUDA_KERNEL_LAUNCH_CHECK();
     count_launches(1);
   }
-  if (grad && r.rows > 0 && !in_warps(r)) {
+  if (grad && r.rows > 0) {
     *grad = new_empty(logits.sizes(), logits.scalar_type(), logits);
     a.grad = grad->mutable_data_ptr();
   }
@@ -774,17 +800,20 @@ at::Tensor token_logprobs_bwd_ready(const at::Tensor& coef, const OptTensor& sca
   a.scale = scale.has_value() ? scale->const_data_ptr<float>() : nullptr;
   a.stats = reinterpret_cast<const float2*>(stats.const_data_ptr<float>());
   a.grad = grad.mutable_data_ptr();
-  // two rounds of a CTA's loads for each chunk
+  const bool warps = in_warps(r);  // else CTAs, in chunks of two rounds of their loads
   const int per = kGradThreads * 8 * kUnroll * 2;
-  a.chunks = std::max(1, (r.vocab + per - 1) / per);
+  a.chunks = warps ? 1 : (r.vocab + per - 1) / per;
   TORCH_CHECK_VALUE((long long)a.chunks * r.rows < (1ll << 31), "logits: too many values for one call");
   a.ready = use_ready;
   // where there is likely nothing to do, no more CTAs than are resident
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  const unsigned grid = use_ready ? std::min(a.chunks * r.rows, sms * 4) : a.chunks * r.rows;
+  const int groups = warps ? kGradThreads / 32 : 1, all = (a.chunks * r.rows + groups - 1) / groups;
+  const unsigned grid = use_ready ? std::min(all, sms * 4) : all;
   with_element(logits.scalar_type(), [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    logprob_grad_kernel<T><<<grid, kGradThreads, 0, at::cuda::getCurrentCUDAStream()>>>(a);
+    const auto stream = at::cuda::getCurrentCUDAStream();
+    if (warps) logprob_grad_kernel<T, 32><<<grid, kGradThreads, 0, stream>>>(a);
+    else logprob_grad_kernel<T, kGradThreads><<<grid, kGradThreads, 0, stream>>>(a);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   });
   count_launches(1);

@@ -12,6 +12,9 @@
 // Queries and keys share one launch. All of it is computed in fp32 and rounded once. Unpacked
 // arithmetic would take longer than the memory: the first and the second values of a lane's four
 // rotated pairs lie in packed registers, two and two, so that nothing is shuffled between them.
+// Measured on one B200: 4096 tokens of 32 + 8 heads of 128 bf16 take 18 us forward (84 MB, 4.7 TB/s)
+// and 31 us backward (126 MB, 4.1 TB/s; 39 us before the arithmetic was packed), and 3 us for the
+// sum of the weights' gradients over the CTAs.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
@@ -368,10 +371,12 @@ Args args_of(Kept& t, const at::Tensor& q, const at::Tensor& k, const at::Tensor
   return a;
 }
 
-// Heads per group: four share a token's angles once there are enough of them to fill the GPU.
+// Heads per group: four share a token's angles (two in the backward pass) once they still fill half the GPU's lanes. 40
+// heads of 128 bf16, forward and backward with one head and with four (two): 8 tokens 2.0 + 3.7 and 2.3 + 3.8 us, 512
+// tokens 4.3 + 6.5 and 3.5 + 6.1 us, 4096 tokens 26 + 42 and 18 + 31 us.
 int heads_per_group(const at::Tensor& q, const at::Tensor& k) {
   const int64_t rows = q.size(0) * q.size(1) * (q.size(2) + k.size(2));
-  const int64_t lanes = (int64_t)at::cuda::getCurrentDeviceProperties()->multiProcessorCount * 1024;
+  const int64_t lanes = (int64_t)at::cuda::getCurrentDeviceProperties()->multiProcessorCount * 512;
   return rows * lanes_per_row(q.size(3)) / 4 >= lanes ? 4 : 1;
 }
 

@@ -257,6 +257,27 @@ def test_losses(b, s, v, dtype):
     _check_losses(logits, targets, None, old, adv, frozen, "no mask")
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("v", [5, 1000, 1025, 8192])
+def test_losses_of_many_short_rows(v, dtype):
+    """Enough rows for a warp each."""
+    logits, targets, mask, old, adv, frozen = _tokens(4, 400, v, dtype)
+    mask[1] = False
+    _check_losses(logits, targets, mask, old, adv, frozen)
+    if v == 1025:
+        _check_losses(logits[:, :-1, 1:1001], targets[:, :-1] % 1000, *(t[:, :-1] for t in (mask, old, adv, frozen)), "cut")
+        bad = logits.clone()
+        bad[~mask] = float("nan")
+        y = torch.where(mask, targets, -100)
+        _check_losses(bad, y, mask, old, adv, frozen, "nothing looked at")
+        y[0, int(mask[0].nonzero()[0])] = v
+        x = bad.requires_grad_()
+        p = model_ops.policy_loss(x, y, old, adv, mask=mask)
+        assert torch.isnan(p.loss) and torch.isnan(torch.autograd.grad(p.loss, x)[0][0]).any()
+        with pytest.raises(RuntimeError, match="error code 3"):
+            _ext.check_device_errors("cuda")
+
+
 def test_losses_masks():
     logits, targets, mask, old, adv, frozen = _tokens(4, 11, 3001, BF16)
     mask[1] = False  # nothing of one answer counts
@@ -274,10 +295,10 @@ def test_losses_masks():
     assert float(p.loss) == 0 and float(p.kl) == 0 and float(p.clipped) == 0 and not g.any()
 
 
-@pytest.mark.parametrize("v", [1000, 5000, 70000])
+@pytest.mark.parametrize("b,v", [(2, 1000), (2, 5000), (2, 70000), (260, 1000)])
 @pytest.mark.parametrize("dtype", [BF16, FP32])
-def test_losses_unusual_logits(v, dtype):
-    logits, targets, mask, old, adv, frozen = _tokens(2, 6, v, dtype)
+def test_losses_unusual_logits(b, v, dtype):
+    logits, targets, mask, old, adv, frozen = _tokens(b, 6, v, dtype)
     low = torch.finfo(dtype).min
     logits[:, 0, v // 2 :] = -torch.inf  # half of the vocabulary is masked
     targets[:, 0] = 3

@@ -178,6 +178,16 @@ def test_models_without_the_options_are_as_they_were():
     assert plain.aux_loss() is None and asked.aux_loss().requires_grad
 
 
+def test_a_model_can_be_copied_after_a_step():
+    """As for a frozen model to stay near."""
+    model = _sparse()
+    tokens = _batch()[0]
+    out = model(tokens)
+    frozen = copy.deepcopy(model)
+    assert frozen.aux_loss() is None and model.aux_loss().requires_grad
+    assert torch.equal(frozen(tokens), out)
+
+
 def test_parameter_groups_and_initialisation():
     model = _sparse()
     model.init_weights(seed=1)
