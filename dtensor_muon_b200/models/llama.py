@@ -10,7 +10,7 @@ DTensor tensor-parallel plans apply without adapters.
 
 from __future__ import annotations
 
-from dataclasses import dataclass, replace
+from dataclasses import dataclass, field, replace
 
 import torch
 import torch.nn.functional as F
@@ -31,7 +31,8 @@ class LlamaConfig:
     rope_theta: float = 500000.0
     max_seq_len: int = 4096
     init_std: float = 0.02
-    qk_norm: bool = False  # RMS norm of every query and key head, in one pass with the rotation
+    # RMS norm of every query and key head, in one pass with the rotation
+    qk_norm: bool = field(default=False, kw_only=True)
 
     @property
     def head_dim(self) -> int:

@@ -41,6 +41,7 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as F
 from torch import Tensor
+from torch._subclasses.fake_tensor import FakeTensor
 
 from . import _ext
 
@@ -203,6 +204,11 @@ def _require(ok: bool, message: str) -> None:
         raise ValueError(message)
 
 
+def _has_values(x: Tensor) -> bool:
+    """Whether ``x``'s values can be looked at: a tracer's tensors have none."""
+    return not (torch.compiler.is_compiling() or isinstance(x, FakeTensor) or x.is_meta)
+
+
 def _wide(x: Tensor) -> Tensor:
     return x if x.dtype == torch.float64 else x.float()
 
@@ -230,7 +236,7 @@ def qk_norm_rope_composition(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: T
     else:
         _require(positions.dtype in (torch.int64, torch.int32) and positions.shape == q.shape[:2],
                  "positions: int64 or int32 [batch, seq] expected")
-        if positions.numel():
+        if _has_values(positions):
             _require(bool(((positions >= 0) & (positions < cos.shape[0])).all()), "positions: a row of cos and sin expected")
         c, s = cos[positions.long()][:, :, None], sin[positions.long()][:, :, None]
     c, s = c.detach(), s.detach()
@@ -300,8 +306,9 @@ def _check_tokens(logits: Tensor, targets: Tensor, mask: Tensor | None) -> None:
     if mask is not None:
         _require(mask.dtype == torch.bool and mask.shape == targets.shape,
                  "mask: bool tensor of the targets' shape on their device expected")
-    inside = (targets >= 0) & (targets < logits.shape[-1])
-    _require(bool((inside if mask is None else inside | ~mask).all()), "targets: a row of the vocabulary expected")
+    if _has_values(targets):
+        inside = (targets >= 0) & (targets < logits.shape[-1])
+        _require(bool((inside if mask is None else inside | ~mask).all()), "targets: a row of the vocabulary expected")
 
 
 def _row_values(v: Tensor, targets: Tensor, name: str) -> Tensor:

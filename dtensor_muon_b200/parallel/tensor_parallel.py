@@ -43,7 +43,7 @@ def apply_tensor_parallel(model: nn.Module, tp_mesh) -> nn.Module:
         att = block.attention
         if att.n_heads % tp or att.n_kv_heads % tp:
             raise ValueError(f"{att.n_heads} heads / {att.n_kv_heads} kv heads do not split over tp={tp}")
-        if tp > 1 and att.q_norm is not None:
+        if tp > 1 and getattr(att, "q_norm", None) is not None:
             # each rank would see the gradient of its own heads only, and the replicated weights would part
             raise ValueError("qk_norm does not split over tensor-parallel ranks")
         parallelize_module(block, tp_mesh, tp_plan(block))

@@ -20,6 +20,7 @@ import torch.distributed as dist
 from torch import Tensor, nn
 
 from .models.llama import Llama, LlamaConfig, lm_loss, muon_and_adam_params
+from .models.mixtral import Mixtral
 from .ops import model_ops
 from .ops.model_ops import PolicyLoss, PreferenceLoss
 from .optim import Muon
@@ -137,9 +138,9 @@ def synthetic_batch(batch: int, seq: int, vocab: int, generator: torch.Generator
 class Trainer:
     """forward -> loss -> backward -> optimizer.step -> zero_grad.
 
-    Every kind of step adds the model's ``aux_loss()`` (the router losses of a
-    sparse model that asks for them) to what it differentiates, and returns the
-    objective without it.
+    Every kind of step adds ``Mixtral.aux_loss()`` (the router losses, where the
+    config asks for them) to what it differentiates, and returns the objective
+    without it.
     """
 
     def __init__(self, model: nn.Module, optimizer: torch.optim.Optimizer):
@@ -147,7 +148,8 @@ class Trainer:
         self.optimizer = optimizer
 
     def _backward(self, loss: Tensor) -> None:
-        aux = self.model.aux_loss() if hasattr(self.model, "aux_loss") else None
+        model = getattr(self.model, "module", self.model)  # past a data-parallel wrapper
+        aux = model.aux_loss() if isinstance(model, Mixtral) else None
         (loss if aux is None else loss + aux).backward()
 
     def _update(self) -> None:

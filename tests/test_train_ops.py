@@ -264,3 +264,40 @@ def test_schemas_and_fake_kernels():
         real = op(*args)
         meta = op(*(a.to("meta") if isinstance(a, torch.Tensor) else a for a in args))
         assert [(m.shape, m.dtype) for m in meta] == [(r.shape, r.dtype) for r in real], op
+
+
+def _all_ops():
+    q, k, wq, wk, cos, sin, _, _ = qk_inputs()
+    logits, targets, mask, old, adv, frozen = token_inputs()
+    ops = torch.ops.dmb
+    return [
+        (ops.qk_norm_rope.default, (q, k, wq, wk, cos, sin, torch.zeros(2, 7, dtype=torch.int64), 1e-5)),
+        (ops.route.default, (logits[0], 2, mask[0])),
+        (ops.token_logprobs.default, (logits, targets, mask)),
+        (ops.policy_loss.default, (logits, targets, old, adv, frozen, mask, 0.2, 0.2, 0.1)),
+        (ops.preference_loss.default, (logits, targets, frozen, mask, 0.1, 0.0)),
+    ]
+
+
+@pytest.mark.parametrize("i", range(5))
+def test_opcheck(i):
+    op, args = _all_ops()[i]
+    args = tuple(a.requires_grad_() if isinstance(a, torch.Tensor) and j == 0 else a for j, a in enumerate(args))
+    torch.library.opcheck(op, args, test_utils=("test_schema", "test_faketensor"))
+
+
+def test_compiled_on_the_cpu():
+    q, k, wq, wk, cos, sin, _, _ = qk_inputs()
+    logits, targets, mask, old, adv, frozen = token_inputs()
+
+    def fn(x, q):
+        a = model_ops.policy_loss(x, targets, old, adv, ref_logp=frozen, mask=mask, kl_coef=0.1).loss
+        b = model_ops.preference_loss(x, targets, frozen, mask=mask).loss
+        c = model_ops.route(x[0], 2, mask=mask[0]).balance + model_ops.token_logprobs(x, targets).sum()
+        return a + b + c + model_ops.qk_norm_rope(q, k, wq, wk, cos, sin)[0].square().mean()
+
+    want, got = ([t.detach().requires_grad_() for t in (logits, q)] for _ in range(2))
+    fn(*want).backward()
+    torch.compile(fn, backend="aot_eager", fullgraph=True)(*got).backward()
+    for w, g in zip(want, got):
+        torch.testing.assert_close(w.grad, g.grad, rtol=1e-5, atol=1e-7)

@@ -8,7 +8,7 @@ import torch
 import torch.nn.functional as F
 
 from dtensor_muon_b200.models.llama import Llama, preset
-from dtensor_muon_b200.models.mixtral import Mixtral, mixtral_preset
+from dtensor_muon_b200.models.mixtral import Mixtral, MixtralConfig, mixtral_preset
 from dtensor_muon_b200.ops import _ext, model_ops
 from dtensor_muon_b200.train import Trainer, build_optimizer
 
@@ -76,7 +76,7 @@ def _by_hand(model, tokens):
 def _grads(model, loss):
     model.zero_grad()
     loss.backward()
-    return {n: p.grad.clone() for n, p in model.named_parameters()}
+    return {n: p.grad.clone() for n, p in model.named_parameters() if p.grad is not None}
 
 
 def _near(got, want, rel):
@@ -154,6 +154,22 @@ def _steps(device, dtype):
     assert all(p.grad is None for p in model.parameters())
 
 
+def test_every_step_adds_the_router_losses():
+    """With an objective that has no gradient, what is left is theirs."""
+    model = _sparse()
+    trainer = Trainer(model, torch.optim.SGD(model.parameters(), lr=0.0))
+    tokens, targets, mask, adv = _batch()
+    model(tokens)
+    want = _grads(model, model.aux_loss())
+    model.zero_grad()
+    seen = {}
+    for n, p in model.named_parameters():
+        p.register_post_accumulate_grad_hook(lambda q, n=n: seen.__setitem__(n, q.grad.clone()))
+    out = trainer.policy_step(tokens, targets, torch.zeros_like(adv), torch.zeros_like(adv), mask=mask)
+    assert float(out.loss) == 0
+    _near({n: seen[n] for n in want}, want, 1e-5)
+
+
 def test_trainer_steps():
     _steps("cpu", torch.float32)
 
@@ -167,6 +183,8 @@ def test_trainer_steps_gpu():
 def test_models_without_the_options_are_as_they_were():
     cfg = preset("tiny", vocab_size=64, n_layers=1)
     assert not cfg.qk_norm
+    by_place = MixtralConfig(512, 128, 2, 4, 4, 128, 1e-5, 1e4, 512, 0.02, 4, 1)
+    assert (by_place.n_experts, by_place.top_k) == (4, 1)
     names = {n for n, _ in Llama(cfg).named_parameters()}
     assert not any("q_norm" in n for n in names)
     plain = Mixtral(mixtral_preset("mixtral-tiny", **SMALL))
