@@ -494,6 +494,7 @@ __device__ __forceinline__ double block_sum(double v, double* smem) {
 __global__ void __launch_bounds__(kReduceThreads) count_kernel(const bool* mask, int rows, int* count) {
   __shared__ double smem[32];
   double n = 0;
+#pragma unroll 8
   for (int i = threadIdx.x; i < rows; i += kReduceThreads) n += mask[i] ? 1 : 0;
   n = block_sum(n, smem);
   if (threadIdx.x == 0) *count = (int)n;
@@ -503,6 +504,7 @@ __global__ void __launch_bounds__(kReduceThreads) count_kernel(const bool* mask,
 __global__ void __launch_bounds__(kReduceThreads) policy_reduce_kernel(const RowArgs a, float* loss, float* kl, float* clipped) {
   __shared__ double smem[32];
   double l = 0, d = 0, c = 0;
+#pragma unroll 4
   for (int i = threadIdx.x; i < a.rows; i += kReduceThreads) {
     l += a.row_loss[i];
     d += a.row_kl[i];
@@ -528,6 +530,7 @@ __global__ void __launch_bounds__(kReduceThreads) preference_reduce_kernel(const
   const int lane = threadIdx.x & 31;
   for (int i = threadIdx.x >> 5; i < 2 * pairs; i += kReduceThreads / 32) {
     double v = 0;
+#pragma unroll 8
     for (int t = lane; t < seq; t += 32) v += diff[(long long)i * seq + t];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
@@ -689,7 +692,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
   const auto ref = ref_logp.has_value() ? ref_logp->contiguous() : at::Tensor();
   const auto m = mask.has_value() ? mask->contiguous() : at::Tensor();
   auto loss = new_empty({}, at::kFloat, logits), kl = new_empty({}, at::kFloat, logits), clipped = new_empty({}, at::kFloat, logits);
-  auto logp = new_empty(targets.sizes(), at::kFloat, logits), coef = new_empty(targets.sizes(), at::kFloat, logits), stats = new_empty({r.rows, 2}, at::kFloat, logits);
+  auto logp = new_empty(targets.sizes(), at::kFloat, logits), coef = new_empty(targets.sizes(), at::kFloat, logits);
+  auto stats = new_empty({r.rows, 2}, at::kFloat, logits);
   // loss and KL of each row, whether it is clipped, and the number of rows that count
   auto work = new_empty({2 * (int64_t)r.rows + 1 + (r.rows + 3) / 4}, at::kFloat, logits);
   RowArgs a = {};
@@ -807,8 +811,8 @@ at::Tensor token_logprobs_bwd_ready(const at::Tensor& coef, const OptTensor& sca
   a.ready = use_ready;
   // where there is likely nothing to do, no more CTAs than are resident
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  const int groups = warps ? kGradThreads / 32 : 1, all = (a.chunks * r.rows + groups - 1) / groups;
-  const unsigned grid = use_ready ? std::min(all, sms * 4) : all;
+  const unsigned groups = warps ? kGradThreads / 32 : 1, all = ((unsigned)(a.chunks * r.rows) + groups - 1) / groups;
+  const unsigned grid = use_ready ? std::min(all, (unsigned)sms * 4) : all;
   with_element(logits.scalar_type(), [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     const auto stream = at::cuda::getCurrentCUDAStream();

@@ -13,8 +13,8 @@
 // arithmetic would take longer than the memory: the first and the second values of a lane's four
 // rotated pairs lie in packed registers, two and two, so that nothing is shuffled between them.
 // Measured on one B200: 4096 tokens of 32 + 8 heads of 128 bf16 take 18 us forward (84 MB, 4.7 TB/s)
-// and 31 us backward (126 MB, 4.1 TB/s; 39 us before the arithmetic was packed), and 3 us for the
-// sum of the weights' gradients over the CTAs.
+// and 25 us backward (126 MB, 5.0 TB/s; 39 us before the arithmetic was packed, 31 before the loads
+// ran ahead of it), and 3 us for the sum of the weights' gradients over the CTAs.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
@@ -132,21 +132,32 @@ __device__ __forceinline__ float row_sum(float v) {
 }
 
 // The lane's four cosines and sines of a token. A position outside the table makes the token's rows NaN and is reported.
-__device__ __forceinline__ Turn load_turn(const Args& a, unsigned token, unsigned s, int at, bool active) {
-  float4 c = make_float4(0.f, 0.f, 0.f, 0.f), sn = c;
+struct Angles {
+  float4 cos, sin;
+};
+
+__device__ __forceinline__ Angles load_angles(const Args& a, unsigned token, unsigned s, int at, bool active) {
+  Angles r;
+  r.cos = r.sin = make_float4(0.f, 0.f, 0.f, 0.f);
   if (active) {
     long long pos = s;
     if (a.positions) pos = a.wide_positions ? static_cast<const int64_t*>(a.positions)[token] : static_cast<const int*>(a.positions)[token];
     if (pos < 0 || pos >= a.table) {
       atomicExch(a.error, (int)kErrBadIndex);
-      c = sn = make_float4(NAN, NAN, NAN, NAN);
+      r.cos = r.sin = make_float4(NAN, NAN, NAN, NAN);
     } else {
       const long long row = pos * (a.dim / 2) + at / 2;
-      c = __ldg(reinterpret_cast<const float4*>(a.cos + row));
-      sn = __ldg(reinterpret_cast<const float4*>(a.sin + row));
+      r.cos = __ldg(reinterpret_cast<const float4*>(a.cos + row));
+      r.sin = __ldg(reinterpret_cast<const float4*>(a.sin + row));
     }
   }
-  return Turn{{f2(c.x, c.y), f2(c.z, c.w)}, {f2(sn.x, sn.y), f2(sn.z, sn.w)}, {f2(-sn.x, -sn.y), f2(-sn.z, -sn.w)}};
+  return r;
+}
+
+__device__ __forceinline__ Turn turn_of(const Angles& g) {
+  return Turn{{f2(g.cos.x, g.cos.y), f2(g.cos.z, g.cos.w)},
+              {f2(g.sin.x, g.sin.y), f2(g.sin.z, g.sin.w)},
+              {f2(-g.sin.x, -g.sin.y), f2(-g.sin.z, -g.sin.w)}};
 }
 
 // A run of up to HPG heads of one token, by one group of LPR lanes.
@@ -168,7 +179,7 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const Args a) {
 #pragma unroll
   for (int i = 0; i < HPG; ++i)
     if (i < n) raw[i] = load_raw8<T>(x + i * h.xh);
-  const Turn turn = load_turn(a, token, s, at, active);
+  const Turn turn = turn_of(load_angles(a, token, s, at, active));
   Pairs w = no_pairs();
   if (active) w = to_pairs<TW>(load_raw8<TW>(static_cast<const TW*>(h.weight) + at));
   const float inv_dim = 1.f / a.dim;
@@ -187,11 +198,13 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const Args a) {
   }
 }
 
-// Each group walks over runs of heads, first of the queries and then of the keys, and keeps its
-// share of the weights' gradients in registers. The CTA joins its groups' shares in a fixed order.
+// Each group walks over runs of heads, first of the queries and then of the keys, and keeps its share of the weights'
+// gradients in registers; the CTA joins its groups' shares in a fixed order. While a lane computes, its next run's values
+// are on their way into its own slots of shared memory, which take no registers and need no barrier.
 template <typename T, typename TW, int LPR, int HPG>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3) bwd_kernel(const Args a) {
-  constexpr int kGroups = kThreads / LPR;
+  constexpr int kGroups = kThreads / LPR, kWords = sizeof(T) / 2;
+  extern __shared__ __align__(16) uint4 slots[];  // [2][HPG][x, dy][kWords][kThreads]
   const int at = (threadIdx.x % LPR) * 8;
   const bool lane_in = at < a.dim;
   const float inv_dim = 1.f / a.dim;
@@ -199,33 +212,61 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3) bwd_kernel(c
 #pragma unroll 1
   for (int part = 0; part < 2; ++part) {
     const Heads& h = a.part[part];
-    const unsigned units = a.tokens * h.chunks.d;
+    const unsigned units = a.tokens * h.chunks.d, step = gridDim.x * kGroups;
     Pairs w = no_pairs(), dw = no_pairs();
     if (lane_in) w = to_pairs<TW>(load_raw8<TW>(static_cast<const TW*>(h.weight) + at));
-    for (unsigned base = blockIdx.x * kGroups; base < units; base += gridDim.x * kGroups) {
-      const unsigned group = base + threadIdx.x / LPR;
+    Angles angles;
+    long long next_out = 0;
+    int next_n = 0;
+    auto fetch = [&](unsigned group, int slot) {
       const bool active = group < units && lane_in;
       const unsigned unit = group < units ? group : 0;
       const unsigned token = h.chunks.div(unit), chunk = unit - token * h.chunks.d;
-      const int h0 = (int)(chunk * HPG), n = active ? min(HPG, h.heads - h0) : 0;
+      const int h0 = (int)(chunk * HPG);
       const unsigned b = a.seq.div(token), s = token - b * a.seq.d;
+      next_n = active ? min(HPG, h.heads - h0) : 0;
+      next_out = ((long long)token * h.heads + h0) * a.dim + at;
       const T* x = static_cast<const T*>(h.x) + b * h.xb + s * h.xs + h0 * h.xh + at;
       const T* dy = static_cast<const T*>(h.dy) + b * h.yb + s * h.ys + h0 * h.yh + at;
-      T* out = static_cast<T*>(h.out) + ((long long)token * h.heads + h0) * a.dim + at;
-      Raw8<T> rx[HPG], ry[HPG];
+      const uint32_t to = smem_u32(slots + (slot * HPG * 2 * kWords) * kThreads + threadIdx.x);
 #pragma unroll
       for (int i = 0; i < HPG; ++i)
-        if (i < n) {
-          rx[i] = load_raw8<T>(x + i * h.xh);
-          ry[i] = load_raw8<T>(dy + i * h.yh);
+        if (i < next_n) {
+#pragma unroll
+          for (int k = 0; k < kWords; ++k) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + ((i * 2) * kWords + k) * kThreads * 16),
+                         "l"(reinterpret_cast<const uint4*>(x + i * h.xh) + k)
+                         : "memory");
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + ((i * 2 + 1) * kWords + k) * kThreads * 16),
+                         "l"(reinterpret_cast<const uint4*>(dy + i * h.yh) + k)
+                         : "memory");
+          }
         }
-      const Turn turn = load_turn(a, token, s, at, active);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      angles = load_angles(a, token, s, at, active);
+    };
+    unsigned group = blockIdx.x * kGroups + threadIdx.x / LPR;
+    int slot = 0;
+    fetch(group, 0);
+    for (unsigned base = blockIdx.x * kGroups; base < units; base += step, group += step, slot ^= 1) {
+      const Turn turn = turn_of(angles);
+      const int n = next_n;
+      T* out = static_cast<T*>(h.out) + next_out;
+      fetch(group + step, slot ^ 1);
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      const uint4* from = slots + (slot * HPG * 2 * kWords) * kThreads + threadIdx.x;
 #pragma unroll
       for (int i = 0; i < HPG; ++i) {
         Pairs v = no_pairs(), g = no_pairs(), u;
         if (i < n) {
-          v = to_pairs<T>(rx[i]);
-          g = rotate(to_pairs<T>(ry[i]), turn.cos, turn.minus, turn.sin);
+          Raw8<T> rx, ry;
+#pragma unroll
+          for (int k = 0; k < kWords; ++k) {
+            rx.w[k] = from[((i * 2) * kWords + k) * kThreads];
+            ry.w[k] = from[((i * 2 + 1) * kWords + k) * kThreads];
+          }
+          v = to_pairs<T>(rx);
+          g = rotate(to_pairs<T>(ry), turn.cos, turn.minus, turn.sin);
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -247,6 +288,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3) bwd_kernel(c
         if (i < n) store_pairs<T>(out + (long long)i * a.dim, v);
       }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (a.partial) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -373,7 +415,7 @@ Args args_of(Kept& t, const at::Tensor& q, const at::Tensor& k, const at::Tensor
 
 // Heads per group: four share a token's angles (two in the backward pass) once they still fill half the GPU's lanes. 40
 // heads of 128 bf16, forward and backward with one head and with four (two): 8 tokens 2.0 + 3.7 and 2.3 + 3.8 us, 512
-// tokens 4.3 + 6.5 and 3.5 + 6.1 us, 4096 tokens 26 + 42 and 18 + 31 us.
+// tokens 4.3 + 6.5 and 3.5 + 6.1 us, 4096 tokens 26 + 42 and 18 + 31 us (before the backward's loads ran ahead).
 int heads_per_group(const at::Tensor& q, const at::Tensor& k) {
   const int64_t rows = q.size(0) * q.size(1) * (q.size(2) + k.size(2));
   const int64_t lanes = (int64_t)at::cuda::getCurrentDeviceProperties()->multiProcessorCount * 512;
@@ -395,6 +437,12 @@ void with_types(const at::Tensor& q, const at::Tensor& w, F&& f) {
     if (w.scalar_type() == at::kFloat) return lanes(static_cast<float*>(nullptr));
     if constexpr (!std::is_same<T, float>::value) lanes(static_cast<T*>(nullptr));
   });
+}
+
+template <typename K>
+void launch_bwd(K kernel, const Args& a, int ctas, size_t slots, cudaStream_t stream) {
+  if (slots > 48 * 1024) C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)slots));
+  kernel<<<ctas, kThreads, slots, stream>>>(a);
 }
 
 }  // namespace
@@ -470,8 +518,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_bwd(
     using TW = std::remove_pointer_t<decltype(tw)>;
     constexpr int L = decltype(lanes)::value;
     const auto stream = at::cuda::getCurrentCUDAStream();
-    if (hpg == 2) bwd_kernel<T, TW, L, 2><<<ctas, kThreads, 0, stream>>>(a);
-    else bwd_kernel<T, TW, L, 1><<<ctas, kThreads, 0, stream>>>(a);
+    const size_t slots = 2 * (size_t)hpg * 2 * kThreads * 8 * sizeof(T);  // up to 64 KB, for fp32
+    if (hpg == 2) launch_bwd(bwd_kernel<T, TW, L, 2>, a, ctas, slots, stream);
+    else launch_bwd(bwd_kernel<T, TW, L, 1>, a, ctas, slots, stream);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
     if (weight_grads) {
       weight_grad_kernel<TW><<<2 * a.dim / 8, kThreads, 0, stream>>>(

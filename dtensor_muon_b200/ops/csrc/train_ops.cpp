@@ -4,6 +4,7 @@
 // autograd function calls its operators through the dispatcher, so that tracers see them.
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
@@ -179,8 +180,11 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> policy_loss_autograd(
   const auto keys = logits.key_set();
   const bool plain = !keys.has(c10::DispatchKey::Python) && !keys.has(c10::DispatchKey::Functionalize) &&
                      !c10::impl::TorchDispatchModeTLS::any_modes_set();
-  const bool grad_now = plain && at::GradMode::is_enabled() && logits.requires_grad() &&
-                        c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None;
+  bool grad_now = plain && at::GradMode::is_enabled() && logits.requires_grad();
+  if (grad_now) {
+    const c10::cuda::CUDAGuard guard(logits.device());
+    grad_now = c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None;
+  }
   auto r = PolicyLoss::apply(logits, targets, old_logp, advantages, ref_logp, mask, clip_low, clip_high, kl_coef, grad_now);
   return {r[0], r[1], r[2], r[3], r[4], r[5]};
 }

@@ -139,6 +139,9 @@ def policy_loss(logits: Tensor, targets: Tensor, old_logp: Tensor, advantages: T
     Mean over the tokens that ``mask`` keeps of ``-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef *
     (exp(d) - 1 - d)`` with ``r = exp(logp - old_logp)`` and ``d = ref_logp - logp``; 0 where it keeps none.
     ``old_logp``, ``advantages`` and ``ref_logp`` are fp32 of the targets' shape, as :func:`token_logprobs` gives them.
+
+    Where the logits need a gradient, the kernel writes it in the same pass, for a loss gradient of 1, and holds it for
+    the backward pass; one of another value (a loss that is divided before ``backward``) is computed anew there.
     """
     args = (logits, targets, old_logp, advantages, ref_logp, mask, clip_low, clip_high, kl_coef)
     if _kernel(logits):
