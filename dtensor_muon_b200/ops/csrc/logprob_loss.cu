@@ -17,12 +17,12 @@
 // would be what is lost. Rows that do not count are not read.
 //
 // Bound by memory, with the exponentials (16 a cycle and SM) close behind: arithmetic is packed,
-// two fp32 values to an instruction. Measured on one B200, alone on the device (6.45 TB/s copied):
-//   scoring 4096 rows of 32000 bf16        47 us, 5.6 TB/s (262 MB)
+// two fp32 values to an instruction, and 16-bit logits are added to fp32 without unpacking. Measured on one B200, alone on the device (6.45 TB/s copied):
+//   scoring 4096 rows of 32000 bf16        46 us, 5.7 TB/s (262 MB)
 //   policy loss and gradient, 4096 rows of 128256 bf16, a quarter masked
-//                                         358 us, 5.1 TB/s (1.84 GB; two passes took 448)
+//                                         355 us, 5.2 TB/s (1.84 GB; two passes took 448)
 //   preference loss and gradient, 4096 rows of 32000 bf16, 40 % masked
-//                                         107 us, 5.4 TB/s (577 MB: the logits are read twice, as
+//                                         106 us, 5.4 TB/s (577 MB: the logits are read twice, as
 //                                         a coefficient hangs on the sums of both sequences)
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
@@ -158,14 +158,14 @@ __device__ __forceinline__ void scan_vectors(const Raw8<T> (&raw)[kUnroll], floa
   m = mx;
   // log2 e in 32 bits is 1.3e-8 of itself too small, which shifts every log-probability to the same side by that times its
   // distance from the mean logit; the next larger number is 6.9e-8 too large. One value in eight with that one leaves 3e-9.
-  const F2 neg = f2(-a, -a), c = f2(kLog2e, kLog2e), up = f2(kLog2e, kLog2eUp);
+  const F2 c = f2(kLog2e, kLog2e), up = f2(kLog2e, kLog2eUp);
   F2 sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
     F2 v[4];
-    unpack_f2<T>(raw[u], v);
+    add_f2<T>(raw[u], -a, v);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) sum[k & 1] = sum[k & 1] + ex2((v[k] + neg) * (k == 3 ? up : c));
+    for (int k = 0; k < 4; ++k) sum[k & 1] = sum[k & 1] + ex2(v[k] * (k == 3 ? up : c));
   }
   const float2 x = f2_values(sum[0] + sum[1]);
   s += x.x + x.y;
@@ -258,11 +258,11 @@ __device__ __forceinline__ float target_logit(const RowArgs& a, const T* p, int6
 // Gradient of one vector; `hot` is the target's place in it, if it has one in 0..7.
 template <typename T>
 __device__ __forceinline__ void grad_vector(const Raw8<T>& raw, T* to, bool aligned, float m, float neg, int hot, float c) {
-  const F2 minus = f2(-m, -m), scale = f2(kLog2e, kLog2e), factor = f2(neg, neg);
+  const F2 scale = f2(kLog2e, kLog2e), factor = f2(neg, neg);
   F2 f[4];
-  unpack_f2<T>(raw, f);
+  add_f2<T>(raw, -m, f);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) f[k] = factor * ex2((f[k] + minus) * scale);
+  for (int k = 0; k < 4; ++k) f[k] = factor * ex2(f[k] * scale);
   if ((unsigned)hot < 8u) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) f[k] = f[k] + f2(2 * k == hot ? c : 0.f, 2 * k + 1 == hot ? c : 0.f);

@@ -131,6 +131,33 @@ __device__ __forceinline__ void unpack_f2(const Raw8<T>& r, F2 (&v)[4]) {
   for (int k = 0; k < 4; ++k) v[k] = f2(f[2 * k], f[2 * k + 1]);
 }
 
+// Eight values plus c, as four pairs of neighbours. 16-bit ones are added as they lie in their words, without unpacking.
+template <typename T>
+__device__ __forceinline__ void add_f2(const Raw8<T>& r, float c, F2 (&v)[4]) {
+  if constexpr (sizeof(T) == 4) {
+    unpack_f2<T>(r, v);
+    const F2 cc = f2(c, c);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = v[k] + cc;
+  } else {
+    const uint32_t w[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float lo, hi;
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tadd.rn.f32.bf16 %0, a, %3;\n\tadd.rn.f32.bf16 %1, b, %3;\n\t}"
+            : "=f"(lo), "=f"(hi)
+            : "r"(w[k]), "f"(c));
+      } else {
+        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tadd.rn.f32.f16 %0, a, %3;\n\tadd.rn.f32.f16 %1, b, %3;\n\t}"
+            : "=f"(lo), "=f"(hi)
+            : "r"(w[k]), "f"(c));
+      }
+      v[k] = f2(lo, hi);
+    }
+  }
+}
+
 template <typename T>
 __device__ __forceinline__ Raw8<T> pack_f2(const F2 (&v)[4]) {
   float f[8];
