@@ -32,7 +32,7 @@ constexpr int kThreads = 256;
 // otherwise stand in front of every load.
 struct Divisor {
   unsigned d, mul, shift;
-  explicit Divisor(unsigned by = 1) : d(by), mul(0), shift(0) {
+  Divisor(unsigned by = 1) : d(by), mul(0), shift(0) {
     while ((1ull << shift) < d) ++shift;
     mul = (unsigned)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
   }

@@ -6,9 +6,9 @@
 //   balance = E / (N^2 k) sum_e c_e sum_t p_te   (1 where every expert gets the same),  z = 1/N sum_t lse_t^2
 //   dl = g (dg - g.dg) at the chosen + p (dbalance E / (N^2 k) (c_e - c.p) + dz 2/N lse)
 //
-// Up to 32 experts a row lies on one, two or four lanes, eight logits on each; above, on a warp, two to 16 logits on each
-// lane. The choice takes k rounds of a maximum over the row by (value, index); on a warp a round is one redux over
-// order-preserving integer keys and a ballot, and only the winner's lane looks through its logits. Every group of lanes
+// Up to 64 experts a row lies on one to eight lanes, eight logits on each; above, on a warp, four to 16 logits on each
+// lane. The choice takes k rounds of a maximum over the row by (value, index); on a warp the lanes sort their logits first,
+// and a round is one redux over order-preserving integer keys and a ballot. Every group of lanes
 // walks over rows and keeps its sums of p and its counts in registers; a CTA joins them in a fixed order and writes one
 // part, and a second kernel sums the parts in 64 bits. So nothing that is rounded is summed by atomics, and a run gives
 // the same bits each time. What bounds it: launches for small batches, the instructions of the k rounds for many experts.
@@ -623,9 +623,10 @@ __global__ void __launch_bounds__(kThreads) route_grad_kernel(const Args a) {
 
 // ------------------------------------------------------------------ host
 
-// f(T, LPR, VPL): up to 32 experts as few lanes per row as hold it at eight logits each (a warp has eight rows or more
-// at once), above a warp per row, with as few logits per lane as hold it. (The lanes' form at 128 fp32 experts, top 8:
-// 56 us for 65535 rows against 20 us for the warp's.)
+// f(T, LPR, VPL): up to 64 experts as few lanes per row as hold it at eight logits each, so that a warp has four rows or
+// more at once; above a warp per row, whose rounds are cheaper and whose other work is dearer. 65536 bf16 rows forward +
+// backward, on lanes and on a warp: 64 experts 14 + 12 and 21 + 21 us at top 2, 28 + 19 and 29 + 20 us at top 8; 128
+// experts 27 + 21 and 28 + 24 us at top 2, 56 + 33 and 37 + 24 us at top 8.
 template <typename F>
 void with_layout(const at::Tensor& logits, F&& f) {
   with_element(logits.scalar_type(), [&](auto* t) {
@@ -634,7 +635,7 @@ void with_layout(const at::Tensor& logits, F&& f) {
     if (e <= 8) f(t, integral_constant<int, 1>(), integral_constant<int, 8>());
     else if (e <= 16) f(t, integral_constant<int, 2>(), integral_constant<int, 8>());
     else if (e <= 32) f(t, integral_constant<int, 4>(), integral_constant<int, 8>());
-    else if (e <= 64) f(t, integral_constant<int, 32>(), integral_constant<int, 2>());
+    else if (e <= 64) f(t, integral_constant<int, 8>(), integral_constant<int, 8>());
     else if (e <= 128) f(t, integral_constant<int, 32>(), integral_constant<int, 4>());
     else if (e <= 256) f(t, integral_constant<int, 32>(), integral_constant<int, 8>());
     else f(t, integral_constant<int, 32>(), integral_constant<int, 16>());
@@ -642,7 +643,7 @@ void with_layout(const at::Tensor& logits, F&& f) {
 }
 
 // Values that a lane has next to each other.
-int per_lane(int experts) { return experts <= 32 ? 8 : experts <= 64 ? 2 : experts <= 128 ? 4 : experts <= 256 ? 8 : 16; }
+int per_lane(int experts) { return experts <= 64 ? 8 : experts <= 128 ? 4 : experts <= 256 ? 8 : 16; }
 
 // Whether rows `stride` elements apart can be moved in a lane's whole words, of up to 16 bytes.
 bool whole_words(const void* p, int64_t rows, int64_t stride, int experts, int64_t size) {
