@@ -131,6 +131,21 @@ class FeedForward(nn.Module):
         return self.w2(_model_ops.swiglu(self.w1(x), self.w3(x)))
 
 
+class AuxLayer(nn.Module):
+    """A layer that leaves a loss of its own beside its output: ``aux``, of the last forward, or None."""
+
+    aux: Tensor | None = None
+
+    def __getstate__(self):
+        # a copy of the model takes none of the last forward's graph along
+        return dict(self.__dict__, aux=None)
+
+
+def aux_layers(model: nn.Module) -> list[AuxLayer]:
+    """The layers of ``model`` that leave a loss, whatever ``model`` is wrapped in."""
+    return [m for m in model.modules() if isinstance(m, AuxLayer)]
+
+
 class Block(nn.Module):
     def __init__(self, cfg: LlamaConfig, ffn: nn.Module | None = None):
         super().__init__()
@@ -183,6 +198,12 @@ class Llama(nn.Module):
             h = layer(h, cos, sin)
         return self.output(self.norm(h))
 
+    def aux_loss(self) -> Tensor | None:
+        """Sum of the layers' own losses of the last forward (the router losses of sparse layers, over this rank's
+        tokens); None where no layer has one."""
+        aux = [m.aux for m in aux_layers(self) if m.aux is not None]
+        return torch.stack(aux).sum() if aux else None
+
 
 def lm_loss(logits: Tensor, targets: Tensor) -> Tensor:
     """Next-token cross entropy in fp32 (fused kernel for bf16 CUDA logits)."""
@@ -217,6 +238,7 @@ def flops_per_token(cfg: LlamaConfig, seq_len: int) -> float:
 
 
 __all__ = [
+    "AuxLayer",
     "Block",
     "FeedForward",
     "Llama",
@@ -224,6 +246,7 @@ __all__ = [
     "PRESETS",
     "RMSNorm",
     "apply_rope",
+    "aux_layers",
     "flops_per_token",
     "lm_loss",
     "muon_and_adam_params",

@@ -17,7 +17,7 @@ import torch
 from torch import Tensor, nn
 
 from ..ops import model_ops as _model_ops
-from .llama import Block, Llama, LlamaConfig
+from .llama import AuxLayer, Block, Llama, LlamaConfig
 
 
 @dataclass(frozen=True)
@@ -60,7 +60,7 @@ def expert_ffn(x: Tensor, counts: Tensor, w1: Tensor, w3: Tensor, w2: Tensor) ->
     return _grouped(h, w2, counts)
 
 
-class MoEFeedForward(nn.Module):
+class MoEFeedForward(AuxLayer):
     def __init__(self, cfg: MixtralConfig, ep=None):
         super().__init__()
         self.n_experts = cfg.n_experts
@@ -72,10 +72,6 @@ class MoEFeedForward(nn.Module):
         self.ep = ep  # ExpertParallel or None (all experts local)
         self.balance_coef, self.z_coef = cfg.balance_coef, cfg.z_coef
         self.aux = None  # the last forward's router losses, where a coefficient asks for them
-
-    def __getstate__(self):
-        # a copy of the model takes none of the last forward's graph along
-        return dict(self.__dict__, aux=None)
 
     def route(self, x: Tensor) -> tuple[Tensor, Tensor]:
         logits = self.router(x)
@@ -113,11 +109,6 @@ class Mixtral(Llama):
 
     def __init__(self, cfg: MixtralConfig, ep=None):
         super().__init__(cfg, block_factory=lambda: Block(cfg, ffn=MoEFeedForward(cfg, ep)))
-
-    def aux_loss(self) -> Tensor | None:
-        """Router losses of the last forward, over this rank's tokens; None without ``balance_coef`` and ``z_coef``."""
-        aux = [m.aux for m in self.modules() if isinstance(m, MoEFeedForward) and m.aux is not None]
-        return torch.stack(aux).sum() if aux else None
 
 
 __all__ = ["MIXTRAL_PRESETS", "MixtralConfig", "Mixtral", "MoEFeedForward", "expert_ffn", "mixtral_preset"]

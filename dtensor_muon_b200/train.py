@@ -19,8 +19,7 @@ import torch
 import torch.distributed as dist
 from torch import Tensor, nn
 
-from .models.llama import Llama, LlamaConfig, lm_loss, muon_and_adam_params
-from .models.mixtral import Mixtral
+from .models.llama import AuxLayer, Llama, LlamaConfig, aux_layers, lm_loss, muon_and_adam_params
 from .ops import model_ops
 from .ops.model_ops import PolicyLoss, PreferenceLoss
 from .optim import Muon
@@ -138,19 +137,24 @@ def synthetic_batch(batch: int, seq: int, vocab: int, generator: torch.Generator
 class Trainer:
     """forward -> loss -> backward -> optimizer.step -> zero_grad.
 
-    Every kind of step adds ``Mixtral.aux_loss()`` (the router losses, where the
-    config asks for them) to what it differentiates, and returns the objective
-    without it.
+    Every kind of step adds the router losses of the model's sparse layers
+    (where their config asks for them) to what it differentiates, and returns
+    the objective without them. The layers are looked for in the model that is
+    trained, also inside a compiled or otherwise wrapped one.
     """
 
     def __init__(self, model: nn.Module, optimizer: torch.optim.Optimizer):
         self.model = model
         self.optimizer = optimizer
 
+    def _aux_layers(self) -> list[AuxLayer]:
+        # a wrapper that is no module itself holds its model in ``module``
+        model = self.model if isinstance(self.model, nn.Module) else getattr(self.model, "module", None)
+        return aux_layers(model) if isinstance(model, nn.Module) else []
+
     def _backward(self, loss: Tensor) -> None:
-        model = getattr(self.model, "module", self.model)  # past a data-parallel wrapper
-        aux = model.aux_loss() if isinstance(model, Mixtral) else None
-        (loss if aux is None else loss + aux).backward()
+        aux = [m.aux for m in self._aux_layers() if m.aux is not None]
+        (loss + torch.stack(aux).sum() if aux else loss).backward()
 
     def _update(self) -> None:
         self.optimizer.step()

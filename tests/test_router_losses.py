@@ -1,0 +1,151 @@
+"""The router losses reach the gradient of every step, whatever the trained model is wrapped in."""
+
+import pytest
+import torch
+from test_train_steps import SMALL, _batch, _near, _sparse
+from testkit import run_distributed
+from torch import nn
+
+from dtensor_muon_b200.models.llama import Block, LlamaConfig, lm_loss
+from dtensor_muon_b200.models.mixtral import MixtralConfig, MoEFeedForward, mixtral_preset
+from dtensor_muon_b200.train import Trainer, build_llama
+
+
+def _config(balance_coef=0.5, z_coef=0.1) -> MixtralConfig:
+    return mixtral_preset("mixtral-tiny", qk_norm=True, balance_coef=balance_coef, z_coef=z_coef, **SMALL)
+
+
+def _built(cfg: LlamaConfig, device="cpu", dtype=torch.float32, **kw):
+    """A sparse decoder from the builder that also shards: a ``Llama`` with sparse blocks."""
+    return build_llama(cfg, torch.device(device), dtype, block_factory=lambda: Block(cfg, ffn=MoEFeedForward(cfg)), **kw)
+
+
+@pytest.fixture(autouse=True)
+def _compiled_anew():
+    torch._dynamo.reset()
+
+
+class _Held(nn.Module):
+    def __init__(self, inner):
+        super().__init__()
+        self.inner = inner
+
+    def forward(self, tokens):
+        return self.inner(tokens)
+
+
+class _Plain:
+    """No module itself, as a data-parallel wrapper of another library may be."""
+
+    def __init__(self, module):
+        self.module = module
+
+    def __call__(self, tokens):
+        return self.module(tokens)
+
+
+WRAPPED = {
+    "bare": lambda m: m,
+    "held": _Held,
+    "plain": _Plain,
+    "compiled": lambda m: torch.compile(m, backend="eager"),
+    "compiled and held": lambda m: _Held(torch.compile(m, backend="eager")),
+}
+
+
+def _seen(model):
+    """What each parameter's gradient is at the end of a step's backward pass."""
+    seen = {}
+    for n, p in model.named_parameters():
+        p.register_post_accumulate_grad_hook(lambda q, n=n: seen.__setitem__(n, q.grad.clone()))
+    return seen
+
+
+def _router_gradients(model, tokens):
+    """Of the router losses alone, from the layers' own."""
+    model(tokens)
+    loss = sum(layer.feed_forward.aux for layer in model.layers)
+    params = {n: p for n, p in model.named_parameters()}
+    grads = torch.autograd.grad(loss, list(params.values()), allow_unused=True)
+    return {n: g for n, g in zip(params, grads) if g is not None}
+
+
+def _take(trainer, step, tokens, targets, mask):
+    zero = torch.zeros(tokens.shape, device=tokens.device)
+    if step == "policy_step":  # without advantages the objective has no gradient
+        return trainer.policy_step(tokens, targets, zero, zero, mask=mask).loss
+    if step == "preference_step":  # nor has it where nothing counts
+        return trainer.preference_step(tokens, targets, zero, mask=torch.zeros_like(mask)).loss
+    return trainer.step(tokens, targets)
+
+
+@pytest.mark.parametrize("made", ["mixtral", "build_llama"])
+@pytest.mark.parametrize("wrapped", WRAPPED)
+@pytest.mark.parametrize("step", ["policy_step", "preference_step"])
+def test_every_step_adds_them(made, wrapped, step):
+    model = _sparse() if made == "mixtral" else _built(_config())
+    tokens, targets, mask, _ = _batch()
+    want = _router_gradients(model, tokens)
+    assert any("router" in n and float(g.norm()) > 1e-3 for n, g in want.items())
+    seen = _seen(model)
+    _take(Trainer(WRAPPED[wrapped](model), torch.optim.SGD(model.parameters(), lr=0.0)), step, tokens, targets, mask)
+    # fp32, the same operations: the objective's zeros are all that differs
+    _near({n: seen[n] for n in want}, want, 1e-5)
+
+
+@pytest.mark.parametrize("wrapped", WRAPPED)
+def test_the_language_model_step_adds_them(wrapped):
+    model = _built(_config())
+    tokens, targets, _, _ = _batch()
+    loss = lm_loss(model(tokens), targets) + sum(layer.feed_forward.aux for layer in model.layers)
+    loss.backward()
+    want = {n: p.grad.clone() for n, p in model.named_parameters()}
+    model.zero_grad()
+    out = Trainer(WRAPPED[wrapped](model), None).forward_backward(tokens, targets)
+    _near({n: p.grad for n, p in model.named_parameters()}, want, 1e-5)
+    assert float(out) < float(loss.detach())  # the objective alone
+
+
+def test_the_model_says_them():
+    model, tokens = _built(_config()), _batch()[0]
+    assert model.aux_loss() is None
+    model(tokens)
+    torch.testing.assert_close(model.aux_loss(), sum(layer.feed_forward.aux for layer in model.layers))
+    silent = _built(_config(0.0, 0.0))
+    silent(tokens)
+    assert silent.aux_loss() is None
+
+
+def test_other_callables_are_trained_as_they_are():
+    """A function has no layers to look through, and a foreign model's own ``aux_loss`` is not ours to call."""
+    model = nn.Sequential(nn.Embedding(512, 8), nn.Linear(8, 512))
+    model.aux_loss = lambda: pytest.fail("called")
+    tokens, targets, _, _ = _batch()
+    for m in (model, lambda t: model(t)):
+        model.zero_grad()
+        Trainer(m, None).forward_backward(tokens, targets)
+        assert all(p.grad.any() for p in model.parameters())
+
+
+def _sharded(rank, world, reshard):
+    from torch.distributed.device_mesh import init_device_mesh
+
+    cfg = _config()
+    mesh = init_device_mesh("cpu", (world,))
+    model = _built(cfg, mesh=mesh, fsdp_comm="nccl", reshard_after_forward=reshard)
+    whole = _built(cfg)
+    with torch.no_grad():
+        for p, q in zip(whole.parameters(), model.parameters()):
+            p.copy_(q.full_tensor())
+    batches = [torch.randint(0, 512, (2, 18), generator=torch.Generator().manual_seed(r)) for r in range(world)]
+    each = [_router_gradients(whole, b[:, :-1]) for b in batches]
+    seen = _seen(model)
+    tokens, targets = batches[rank][:, :-1], batches[rank][:, 1:]
+    _take(Trainer(model, torch.optim.SGD(model.parameters(), lr=0.0)), "policy_step", tokens, targets, None)
+    # the ranks' gradients are averaged
+    _near({n: seen[n].full_tensor() for n in each[0]}, {n: sum(e[n] for e in each) / world for n in each[0]}, 1e-5)
+
+
+@pytest.mark.parametrize("reshard", [False, True])
+def test_a_sharded_decoder(reshard):
+    run_distributed(_sharded, 2, args=(reshard,), backend="gloo", device_type="cpu", timeout_s=120)
