@@ -132,7 +132,11 @@ class FeedForward(nn.Module):
 
 
 class AuxLayer(nn.Module):
-    """A layer that leaves a loss of its own beside its output: ``aux``, of the last forward, or None."""
+    """A layer that leaves a loss of its own beside its output: ``aux``, of the last forward, or None.
+
+    ``aux`` holds that forward's graph, and with it the nodes of the leaves, until the next forward or
+    :func:`detach_aux`.
+    """
 
     aux: Tensor | None = None
 
@@ -144,6 +148,14 @@ class AuxLayer(nn.Module):
 def aux_layers(model: nn.Module) -> list[AuxLayer]:
     """The layers of ``model`` that leave a loss, whatever ``model`` is wrapped in."""
     return [m for m in model.modules() if isinstance(m, AuxLayer)]
+
+
+def detach_aux(model: nn.Module) -> None:
+    """Leaves the layers' losses as values without a graph. For after a backward pass: what a graph that is done with
+    holds is freed, and a backward pass may be captured, for which no eager graph of the same leaves may live."""
+    for m in aux_layers(model):
+        if m.aux is not None:
+            m.aux = m.aux.detach()
 
 
 class Block(nn.Module):
@@ -247,6 +259,7 @@ __all__ = [
     "RMSNorm",
     "apply_rope",
     "aux_layers",
+    "detach_aux",
     "flops_per_token",
     "lm_loss",
     "muon_and_adam_params",

@@ -19,7 +19,7 @@ import torch
 import torch.distributed as dist
 from torch import Tensor, nn
 
-from .models.llama import AuxLayer, Llama, LlamaConfig, aux_layers, lm_loss, muon_and_adam_params
+from .models.llama import Llama, LlamaConfig, aux_layers, detach_aux, lm_loss, muon_and_adam_params
 from .ops import model_ops
 from .ops.model_ops import PolicyLoss, PreferenceLoss
 from .optim import Muon
@@ -140,21 +140,26 @@ class Trainer:
     Every kind of step adds the router losses of the model's sparse layers
     (where their config asks for them) to what it differentiates, and returns
     the objective without them. The layers are looked for in the model that is
-    trained, also inside a compiled or otherwise wrapped one.
+    trained, also inside a compiled or otherwise wrapped one. After a step they
+    are values without a graph.
     """
 
     def __init__(self, model: nn.Module, optimizer: torch.optim.Optimizer):
         self.model = model
         self.optimizer = optimizer
 
-    def _aux_layers(self) -> list[AuxLayer]:
-        # a wrapper that is no module itself holds its model in ``module``
+    def _module(self) -> nn.Module:
+        # a wrapper that is no module itself holds its model in ``module``; a function holds none
         model = self.model if isinstance(self.model, nn.Module) else getattr(self.model, "module", None)
-        return aux_layers(model) if isinstance(model, nn.Module) else []
+        return model if isinstance(model, nn.Module) else nn.Module()
 
     def _backward(self, loss: Tensor) -> None:
-        aux = [m.aux for m in self._aux_layers() if m.aux is not None]
-        (loss + torch.stack(aux).sum() if aux else loss).backward()
+        model = self._module()
+        aux = [m.aux for m in aux_layers(model) if m.aux is not None]
+        try:
+            (loss + torch.stack(aux).sum() if aux else loss).backward()
+        finally:
+            detach_aux(model)
 
     def _update(self) -> None:
         self.optimizer.step()

@@ -116,6 +116,51 @@ def test_the_model_says_them():
     assert silent.aux_loss() is None
 
 
+@pytest.mark.parametrize("step", ["step", "policy_step", "preference_step"])
+def test_no_graph_is_left_after_a_step(step):
+    model = _sparse()
+    tokens, targets, mask, _ = _batch()
+    model(tokens)
+    want = model.aux_loss().detach()
+    trainer = Trainer(model, torch.optim.SGD(model.parameters(), lr=0.0))
+    _take(trainer, step, tokens, targets, mask)
+    aux = [layer.feed_forward.aux for layer in model.layers]
+    assert all(a is not None and a.grad_fn is None and not a.requires_grad for a in aux)
+    torch.testing.assert_close(model.aux_loss(), want)  # the value can be logged
+    model(tokens)
+    with pytest.raises(ZeroDivisionError):  # nor after one that fails
+        trainer._backward(_Broken.apply(torch.zeros((), requires_grad=True)))
+    assert all(layer.feed_forward.aux.grad_fn is None for layer in model.layers)
+
+
+class _Broken(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x):
+        return x.clone()
+
+    @staticmethod
+    def backward(ctx, g):
+        raise ZeroDivisionError
+
+
+@pytest.mark.gpu
+def test_a_step_is_captured_after_an_eager_one():
+    model = _sparse("cuda", torch.bfloat16)
+    tokens, targets, _, _ = _batch("cuda")
+    trainer = Trainer(model, None)
+    eager = trainer.forward_backward(tokens, targets)
+    want = {n: p.grad for n, p in model.named_parameters()}
+    model.zero_grad(set_to_none=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = trainer.forward_backward(tokens, targets)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(loss, eager)
+    # the same kernels on the same numbers; sums of rows of one token or expert may come in another order
+    _near({n: p.grad.float() for n, p in model.named_parameters()}, {n: g.float() for n, g in want.items()}, 2**-8)
+
+
 def test_other_callables_are_trained_as_they_are():
     """A function has no layers to look through, and a foreign model's own ``aux_loss`` is not ours to call."""
     model = nn.Sequential(nn.Embedding(512, 8), nn.Linear(8, 512))
