@@ -135,10 +135,20 @@ class AuxLayer(nn.Module):
     """A layer that leaves a loss of its own beside its output: ``aux``, of the last forward, or None.
 
     ``aux`` holds that forward's graph, and with it the nodes of the leaves, until the next forward or
-    :func:`detach_aux`.
+    :func:`detach_aux`. ``aux_graph`` says whether gradients were enabled then: the first forward of a reentrant
+    checkpoint has them off, and its second one comes when the losses have been added up.
     """
 
     aux: Tensor | None = None
+    aux_graph: bool = False
+
+    @property
+    def aux_asked(self) -> bool:
+        """Whether a forward is to leave a loss."""
+        return False
+
+    def leave_aux(self, aux: Tensor) -> None:
+        self.aux, self.aux_graph = aux, torch.is_grad_enabled()
 
     def __getstate__(self):
         # a copy of the model takes none of the last forward's graph along

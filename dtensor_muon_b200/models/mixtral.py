@@ -71,7 +71,10 @@ class MoEFeedForward(AuxLayer):
         self.w2 = nn.Parameter(torch.empty(cfg.n_experts, cfg.dim, cfg.ffn_dim))  # down
         self.ep = ep  # ExpertParallel or None (all experts local)
         self.balance_coef, self.z_coef = cfg.balance_coef, cfg.z_coef
-        self.aux = None  # the last forward's router losses, where a coefficient asks for them
+
+    @property
+    def aux_asked(self) -> bool:  # the router losses
+        return bool(self.balance_coef or self.z_coef)
 
     def route(self, x: Tensor) -> tuple[Tensor, Tensor]:
         logits = self.router(x)
@@ -82,10 +85,10 @@ class MoEFeedForward(AuxLayer):
         B, S, D = x.shape
         flat = x.reshape(-1, D)
         counts = None
-        if self.balance_coef or self.z_coef:
+        if self.aux_asked:
             gates, idx, counts, balance, z = _model_ops.route(self.router(flat), self.top_k)
             gates = gates.to(x.dtype)
-            self.aux = self.balance_coef * balance + self.z_coef * z
+            self.leave_aux(self.balance_coef * balance + self.z_coef * z)
         else:
             idx, gates = self.route(flat)
         w1, w3, w2 = (w.to_local() if hasattr(w, "to_local") else w for w in (self.w1, self.w3, self.w2))

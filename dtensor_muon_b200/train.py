@@ -141,7 +141,8 @@ class Trainer:
     (where their config asks for them) to what it differentiates, and returns
     the objective without them. The layers are looked for in the model that is
     trained, also inside a compiled or otherwise wrapped one. After a step they
-    are values without a graph.
+    are values without a graph. Where a forward leaves none with a gradient (a
+    reentrant checkpoint around a sparse layer) the step raises.
     """
 
     def __init__(self, model: nn.Module, optimizer: torch.optim.Optimizer):
@@ -153,9 +154,19 @@ class Trainer:
         model = self.model if isinstance(self.model, nn.Module) else getattr(self.model, "module", None)
         return model if isinstance(model, nn.Module) else nn.Module()
 
+    def _forward(self, tokens: Tensor) -> Tensor:
+        for m in aux_layers(self._module()):
+            m.aux = None
+        return self.model(tokens)
+
     def _backward(self, loss: Tensor) -> None:
         model = self._module()
-        aux = [m.aux for m in aux_layers(model) if m.aux is not None]
+        layers = aux_layers(model)
+        aux = [m.aux for m in layers if m.aux is not None]
+        asked = [m for m in layers if m.aux_asked and any(p.requires_grad for p in m.parameters())]
+        if any(m.aux is not None and not m.aux_graph for m in asked) or (asked and not aux):
+            raise RuntimeError("the forward left no router losses with a gradient, which balance_coef and z_coef ask for: "
+                               "under activation checkpointing, use_reentrant=False keeps them")
         try:
             (loss + torch.stack(aux).sum() if aux else loss).backward()
         finally:
@@ -166,7 +177,7 @@ class Trainer:
         self.optimizer.zero_grad(set_to_none=True)
 
     def forward_backward(self, tokens: Tensor, targets: Tensor) -> Tensor:
-        loss = lm_loss(self.model(tokens), targets)
+        loss = lm_loss(self._forward(tokens), targets)
         self._backward(loss)
         return loss.detach()
 
@@ -184,7 +195,7 @@ class Trainer:
                     ref_logp: Tensor | None = None, mask: Tensor | None = None, clip_low: float = 0.2,
                     clip_high: float = 0.2, kl_coef: float = 0.0) -> PolicyLoss:
         """One clipped policy step on sampled tokens; arguments as :func:`ops.model_ops.policy_loss`."""
-        out = model_ops.policy_loss(self.model(tokens), targets, old_logp, advantages, ref_logp=ref_logp, mask=mask,
+        out = model_ops.policy_loss(self._forward(tokens), targets, old_logp, advantages, ref_logp=ref_logp, mask=mask,
                                     clip_low=clip_low, clip_high=clip_high, kl_coef=kl_coef)
         self._backward(out.loss)
         self._update()
@@ -194,7 +205,7 @@ class Trainer:
                         beta: float = 0.1, label_smoothing: float = 0.0) -> PreferenceLoss:
         """One step on pairs of answers, the chosen ones in front of the rejected ones; arguments as
         :func:`ops.model_ops.preference_loss`."""
-        out = model_ops.preference_loss(self.model(tokens), targets, ref_logp, mask=mask, beta=beta,
+        out = model_ops.preference_loss(self._forward(tokens), targets, ref_logp, mask=mask, beta=beta,
                                         label_smoothing=label_smoothing)
         self._backward(out.loss)
         self._update()

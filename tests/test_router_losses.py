@@ -1,10 +1,14 @@
 """The router losses reach the gradient of every step, whatever the trained model is wrapped in."""
 
+import copy
+from functools import partial
+
 import pytest
 import torch
 from test_train_steps import SMALL, _batch, _near, _sparse
 from testkit import run_distributed
 from torch import nn
+from torch.utils.checkpoint import checkpoint
 
 from dtensor_muon_b200.models.llama import Block, LlamaConfig, lm_loss
 from dtensor_muon_b200.models.mixtral import MixtralConfig, MoEFeedForward, mixtral_preset
@@ -131,6 +135,62 @@ def test_no_graph_is_left_after_a_step(step):
     with pytest.raises(ZeroDivisionError):  # nor after one that fails
         trainer._backward(_Broken.apply(torch.zeros((), requires_grad=True)))
     assert all(layer.feed_forward.aux.grad_fn is None for layer in model.layers)
+
+
+def _checkpointed(model, reentrant):
+    for layer in model.layers:
+        layer.forward = partial(checkpoint, layer.forward, use_reentrant=reentrant)
+    return model
+
+
+@pytest.mark.parametrize("step", ["step", "policy_step", "preference_step"])
+def test_checkpointed_layers(step):
+    model = _sparse()
+    tokens, targets, mask, _ = _batch()
+    want = _router_gradients(model, tokens)
+    trainer = Trainer(_checkpointed(model, False), torch.optim.SGD(model.parameters(), lr=0.0))
+    if step != "step":
+        seen = _seen(model)
+        _take(trainer, step, tokens, targets, mask)
+        _near({n: seen[n] for n in want}, want, 1e-5)
+    else:
+        trainer.step(tokens, targets)
+    assert all(layer.feed_forward.aux.grad_fn is None for layer in model.layers)
+    # a reentrant one's forward has no gradients: the losses would be lost
+    model = _sparse()
+    trainer = Trainer(_checkpointed(model, True), torch.optim.SGD(model.parameters(), lr=0.0))
+    with pytest.raises(RuntimeError, match="use_reentrant=False"):
+        _take(trainer, step, tokens, targets, mask)
+    assert all(p.grad is None for p in model.parameters())
+    # nothing is lost where nothing is asked for, or where the layers are frozen
+    model = _built(_config(0.0, 0.0))
+    _take(Trainer(_checkpointed(model, True), torch.optim.SGD(model.parameters(), lr=0.0)), step, tokens, targets, mask)
+    model = _sparse()
+    for layer in model.layers:
+        layer.feed_forward.requires_grad_(False)
+    _take(Trainer(_checkpointed(model, True), torch.optim.SGD(model.parameters(), lr=0.0)), step, tokens, targets, mask)
+
+
+def test_a_model_whose_layers_never_ran_is_refused():
+    """As a wrapper that trains a copy: the trained model's layers leave nothing."""
+    model = _sparse()
+    wrapper = _Held(copy.deepcopy(model))
+    wrapper.forward = copy.deepcopy(model).forward
+    tokens, targets, _, _ = _batch()
+    with pytest.raises(RuntimeError, match="router losses"):
+        Trainer(wrapper, None).forward_backward(tokens, targets)
+
+
+def test_a_coefficient_may_change():
+    model = _sparse()
+    tokens, targets, mask, _ = _batch()
+    trainer = Trainer(model, torch.optim.SGD(model.parameters(), lr=0.0))
+    trainer.step(tokens, targets)
+    for layer in model.layers:
+        layer.feed_forward.balance_coef = layer.feed_forward.z_coef = 0.0
+    seen = _seen(model)
+    _take(trainer, "preference_step", tokens, targets, mask)
+    assert model.aux_loss() is None and not any(g.any() for g in seen.values())
 
 
 class _Broken(torch.autograd.Function):
