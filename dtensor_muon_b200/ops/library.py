@@ -344,23 +344,29 @@ def policy_loss_composition(logits: Tensor, targets: Tensor, old_logp: Tensor, a
     _require(kl_coef == 0 or ref_logp is not None, "kl_coef needs ref_logp")
     logp, stats = _logprobs(logits, targets, mask)
     valid = torch.ones_like(targets, dtype=torch.bool) if mask is None else mask
-    zero = torch.zeros((), device=logp.device, dtype=logp.dtype)
+    # 64 bits from here on, as the kernel has it: a ratio of 32 bits is infinite from exp(89) on
+    new, t = logp.double(), logp.dtype
+    zero = torch.zeros((), device=logp.device, dtype=new.dtype)
     n = valid.sum().clamp(min=1)
-    ratio = torch.exp(torch.where(valid, logp - _row_values(old_logp, targets, "old_logp"), zero))
-    adv = torch.where(valid, _row_values(advantages, targets, "advantages").to(logp.dtype), zero)
-    free, held = ratio * adv, ratio.clamp(1 - clip_low, 1 + clip_high) * adv
-    clipped = free > held
+    gap = torch.where(valid, new - _row_values(old_logp, targets, "old_logp"), zero)
+    adv = torch.where(valid, _row_values(advantages, targets, "advantages").double(), zero)
+    ratio = torch.exp(gap.detach())
+    held = ratio.clamp(1 - clip_low, 1 + clip_high) * adv
+    clipped = ratio * adv > held
+    # a clipped token has no gradient, however large its ratio: its exponential is not one that is differentiated
+    free = torch.exp(torch.where(clipped, zero, gap)) * adv
     rows = -torch.where(clipped, held, free)
     coef = torch.where(clipped, zero, -free).detach()
     kl = zero
     if ref_logp is not None:
-        d = torch.where(valid, _row_values(ref_logp, targets, "ref_logp") - logp, zero)
+        d = torch.where(valid, _row_values(ref_logp, targets, "ref_logp") - new, zero)
         k3 = torch.expm1(d) - d
         kl = k3.detach().sum() / n
         if kl_coef != 0:
             rows = rows + kl_coef * k3
             coef = coef - kl_coef * torch.expm1(d.detach())
-    return (rows.sum() / n, logp.detach().clone(), kl.clone(), clipped.to(logp.dtype).sum() / n, stats, coef / n)
+    return ((rows.sum() / n).to(t), logp.detach().clone(), kl.to(t, copy=True), (clipped.sum() / n).to(t), stats,
+            (coef / n).to(t))
 
 
 def preference_loss_composition(logits: Tensor, targets: Tensor, ref_logp: Tensor, mask: Tensor | None, beta: float,
