@@ -209,6 +209,13 @@ def _has_values(x: Tensor) -> bool:
     return not (torch.compiler.is_compiling() or isinstance(x, FakeTensor) or x.is_meta)
 
 
+def _require_all(ok: Tensor, message: str) -> None:
+    # within torch.func.vmap a value of its own for each sample: all of them are looked at
+    while torch._C._functorch.is_functorch_wrapped_tensor(ok):
+        ok = torch._C._functorch.get_unwrapped(ok)
+    _require(bool(ok.all()), message)
+
+
 def _wide(x: Tensor) -> Tensor:
     return x if x.dtype == torch.float64 else x.float()
 
@@ -237,7 +244,7 @@ def qk_norm_rope_composition(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: T
         _require(positions.dtype in (torch.int64, torch.int32) and positions.shape == q.shape[:2],
                  "positions: int64 or int32 [batch, seq] expected")
         if _has_values(positions):
-            _require(bool(((positions >= 0) & (positions < cos.shape[0])).all()), "positions: a row of cos and sin expected")
+            _require_all((positions >= 0) & (positions < cos.shape[0]), "positions: a row of cos and sin expected")
         c, s = cos[positions.long()][:, :, None], sin[positions.long()][:, :, None]
     c, s = c.detach(), s.detach()
 
@@ -274,7 +281,7 @@ def route_composition(logits: Tensor, top_k: int, mask: Tensor | None) -> tuple[
     # tokens that do not count keep their choice and give nothing else, whatever their logits are
     x = torch.where(valid[:, None], _wide(logits), torch.zeros((), device=logits.device, dtype=_wide(logits).dtype))
     gates = torch.softmax(x.gather(1, experts), dim=1) * valid[:, None]
-    chosen = torch.zeros(t, e, dtype=torch.int64, device=logits.device).scatter_(1, experts, 1)
+    chosen = torch.zeros(t, e, dtype=torch.int64, device=logits.device).scatter(1, experts, 1)
     counts = (chosen * valid[:, None]).sum(0)
     n = valid.sum().clamp(min=1).to(x.dtype)
     share = counts.to(x.dtype) / (n * top_k)
@@ -308,7 +315,7 @@ def _check_tokens(logits: Tensor, targets: Tensor, mask: Tensor | None) -> None:
                  "mask: bool tensor of the targets' shape on their device expected")
     if _has_values(targets):
         inside = (targets >= 0) & (targets < logits.shape[-1])
-        _require(bool((inside if mask is None else inside | ~mask).all()), "targets: a row of the vocabulary expected")
+        _require_all(inside if mask is None else inside | ~mask, "targets: a row of the vocabulary expected")
 
 
 def _row_values(v: Tensor, targets: Tensor, name: str) -> Tensor:
