@@ -102,7 +102,7 @@ class Attention(nn.Module):
             q = self.wq(x).view(B, S, -1, self.head_dim)
             k = self.wk(x).view(B, S, -1, self.head_dim)
             v = self.wv(x).view(B, S, -1, self.head_dim)
-        if self.q_norm is not None:
+        if getattr(self, "q_norm", None) is not None:  # a module saved whole before there were head norms has none
             q, k = _model_ops.qk_norm_rope(q, k, self.q_norm.weight, self.k_norm.weight, cos, sin, self.q_norm.eps)
         else:
             q, k = apply_rope(q, cos, sin), apply_rope(k, cos, sin)

@@ -61,6 +61,8 @@ def expert_ffn(x: Tensor, counts: Tensor, w1: Tensor, w3: Tensor, w2: Tensor) ->
 
 
 class MoEFeedForward(AuxLayer):
+    balance_coef = z_coef = 0.0  # what a module saved whole before there were router losses has
+
     def __init__(self, cfg: MixtralConfig, ep=None):
         super().__init__()
         self.n_experts = cfg.n_experts

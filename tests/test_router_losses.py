@@ -1,6 +1,7 @@
 """The router losses reach the gradient of every step, whatever the trained model is wrapped in."""
 
 import copy
+from dataclasses import replace
 from functools import partial
 
 import pytest
@@ -10,7 +11,7 @@ from testkit import run_distributed
 from torch import nn
 from torch.utils.checkpoint import checkpoint
 
-from dtensor_muon_b200.models.llama import Block, LlamaConfig, lm_loss
+from dtensor_muon_b200.models.llama import Attention, Block, LlamaConfig, lm_loss
 from dtensor_muon_b200.models.mixtral import MixtralConfig, MoEFeedForward, mixtral_preset
 from dtensor_muon_b200.train import Trainer, build_llama
 
@@ -191,6 +192,28 @@ def test_a_coefficient_may_change():
     seen = _seen(model)
     _take(trainer, "preference_step", tokens, targets, mask)
     assert model.aux_loss() is None and not any(g.any() for g in seen.values())
+
+
+def test_modules_saved_whole_before_the_options():
+    """Their state has no head norms and no coefficients."""
+    model = _built(_config(0.0, 0.0))
+    plain = _built(replace(_config(0.0, 0.0), qk_norm=False))
+    plain.load_state_dict(model.state_dict(), strict=False)
+    tokens, targets, _, _ = _batch()
+    want = plain(tokens)
+    for layer in plain.layers:
+        state = dict(layer.attention.__dict__)
+        for name in ("q_norm", "k_norm"):
+            del state[name]
+        layer.attention = Attention.__new__(Attention)
+        layer.attention.__setstate__(state)
+        state = dict(layer.feed_forward.__dict__)
+        for name in ("balance_coef", "z_coef", "aux"):
+            state.pop(name, None)
+        layer.feed_forward = MoEFeedForward.__new__(MoEFeedForward)
+        layer.feed_forward.__setstate__(state)
+    assert torch.equal(plain(tokens), want) and plain.aux_loss() is None
+    Trainer(copy.deepcopy(plain), None).forward_backward(tokens, targets)
 
 
 class _Broken(torch.autograd.Function):
