@@ -8,6 +8,8 @@ instead of silently running a PyTorch fallback.
 from __future__ import annotations
 
 import importlib
+import sys
+import types
 
 _C = None
 _IMPORT_ERROR: Exception | None = None
@@ -48,12 +50,22 @@ _LAUNCHES = {
 _proxy_launches = 0
 
 
-def __getattr__(name: str):
-    # launch_count: kernels launched through the bindings (counted by the proxy below) and by the
-    # operators that the extension registers with the dispatcher itself (counted there).
-    if name == "launch_count":
+class _Module(types.ModuleType):
+    """This module, with a counter that can be set (to 0, say) as any other of its names can."""
+
+    @property
+    def launch_count(self) -> int:
+        """Kernels launched through the bindings (counted by the proxy below) and by the operators that the extension
+        registers with the dispatcher itself (counted there)."""
         return _proxy_launches + (_C._mod.launches_counted() if _C is not None else 0)
-    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+    @launch_count.setter
+    def launch_count(self, value: int) -> None:
+        global _proxy_launches
+        _proxy_launches += value - self.launch_count
+
+
+sys.modules[__name__].__class__ = _Module
 
 
 class _Counted:
@@ -108,7 +120,8 @@ def available() -> bool:
 
 
 def check_device_errors(device) -> None:
-    """Raise if a kernel on ``device`` recorded a timed-out wait since the last check."""
+    """Raise if a kernel on ``device`` recorded an error since the last check: a wait that timed out, or an index outside
+    its table."""
     import torch
 
     idx = torch.device(device).index
