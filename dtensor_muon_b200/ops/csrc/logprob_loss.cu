@@ -52,6 +52,13 @@ constexpr int kWarpRows = 4;       // rows of a CTA whose warps have one each
 
 enum Mode { kLogprob, kPolicy, kPreference };
 
+// A row's part of the policy loss. The loss is in 64 bits, as rows may cancel in the sum; 16 bytes for one load.
+struct alignas(16) RowLoss {
+  double loss;
+  float kl;
+  int clipped;
+};
+
 struct RowArgs {
   const void* logits;
   long long stride_b, stride_s;  // elements
@@ -66,8 +73,8 @@ struct RowArgs {
   const float *old_logp, *advantages, *ref_logp;
   double clip_low, clip_high, kl_coef;
   const int* count;  // rows that the mask keeps; null: all
-  float *row_loss, *row_kl, *coef;
-  bool* row_clipped;
+  RowLoss* row_loss;
+  float* coef;
   double* row_diff;
   void* grad;  // contiguous; null: no gradient
 };
@@ -224,9 +231,7 @@ __device__ __forceinline__ float finish_row(const RowArgs& a, int row, float xy,
         coef -= a.kl_coef * e;
       }
     }
-    a.row_loss[row] = (float)loss;
-    a.row_kl[row] = (float)kl;
-    a.row_clipped[row] = clipped;
+    a.row_loss[row] = RowLoss{loss, (float)kl, clipped};
     coef *= a.count ? (*a.count > 0 ? 1.0 / *a.count : 0.0) : 1.0 / a.rows;
     a.coef[row] = (float)coef;
     return (float)coef;
@@ -240,9 +245,7 @@ __device__ __forceinline__ void skip_row(const RowArgs& a, int row) {
   a.logp[row] = 0.f;
   a.stats[row] = make_float2(0.f, 1.f);
   if constexpr (MODE == kPolicy) {
-    a.row_loss[row] = 0.f;
-    a.row_kl[row] = 0.f;
-    a.row_clipped[row] = false;
+    a.row_loss[row] = RowLoss{0.0, 0.f, 0};
     a.coef[row] = 0.f;
   }
   if constexpr (MODE == kPreference) a.row_diff[row] = 0.0;
@@ -508,9 +511,10 @@ __global__ void __launch_bounds__(kReduceThreads) policy_reduce_kernel(const Row
   double l = 0, d = 0, c = 0;
 #pragma unroll 4
   for (int i = threadIdx.x; i < a.rows; i += kReduceThreads) {
-    l += a.row_loss[i];
-    d += a.row_kl[i];
-    c += a.row_clipped[i] ? 1 : 0;
+    const RowLoss r = a.row_loss[i];
+    l += r.loss;
+    d += r.kl;
+    c += r.clipped;
   }
   l = block_sum(l, smem);
   d = block_sum(d, smem);
@@ -696,8 +700,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
   auto loss = new_empty({}, at::kFloat, logits), kl = new_empty({}, at::kFloat, logits), clipped = new_empty({}, at::kFloat, logits);
   auto logp = new_empty(targets.sizes(), at::kFloat, logits), coef = new_empty(targets.sizes(), at::kFloat, logits);
   auto stats = new_empty({r.rows, 2}, at::kFloat, logits);
-  // loss and KL of each row, whether it is clipped, and the number of rows that count
-  auto work = new_empty({2 * (int64_t)r.rows + 1 + (r.rows + 3) / 4}, at::kFloat, logits);
+  // each row's part, and the number of rows that count
+  auto work = new_empty({2 * (int64_t)r.rows + 1}, at::kDouble, logits);
   RowArgs a = {};
   a.targets = t.const_data_ptr<int64_t>();
   a.mask = m.defined() ? m.const_data_ptr<bool>() : nullptr;
@@ -709,10 +713,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
   a.clip_low = clip_low;
   a.clip_high = clip_high;
   a.kl_coef = kl_coef;
-  a.row_loss = work.mutable_data_ptr<float>();
-  a.row_kl = a.row_loss + r.rows;
-  int* count = reinterpret_cast<int*>(a.row_kl + r.rows);
-  a.row_clipped = reinterpret_cast<bool*>(count + 1);
+  a.row_loss = reinterpret_cast<RowLoss*>(work.mutable_data_ptr<double>());
+  int* count = reinterpret_cast<int*>(a.row_loss + r.rows);
   a.coef = coef.mutable_data_ptr<float>();
   const auto stream = at::cuda::getCurrentCUDAStream();
   if (a.mask) {

@@ -57,3 +57,19 @@ def test_equal_logits_are_exact(rows, vocab):
     y = torch.zeros(rows, dtype=torch.int64, device="cuda")
     want = torch.tensor(-math.log(vocab), dtype=torch.float64).float().item()
     assert set(model_ops.token_logprobs(x, y).tolist()) == {want}
+
+
+@pytest.mark.parametrize("n,vocab", [(1, 64), (400, 64), (2, 65536)])
+def test_losses_that_cancel(n, vocab):
+    """Pairs of tokens whose losses cancel to a rounding of the advantage: nothing of a token's loss is lost before the sum."""
+    logits = torch.zeros(n, 2, vocab, device="cuda", requires_grad=True)
+    targets = torch.zeros(n, 2, dtype=torch.int64, device="cuda")
+    old = (-math.log(vocab) - torch.tensor([0.09, -0.11], device="cuda")).expand(n, 2)
+    ratio = torch.exp(-math.log(vocab) - old.double())  # the logits are alike: a log-probability has no error
+    adv = torch.stack([torch.ones(n, device="cuda"), -(ratio[:, 0] / ratio[:, 1]).float()], 1)
+    want = -(ratio * adv.double()).mean()
+    assert 0 < abs(float(want)) < 1e-7
+    p = model_ops.policy_loss(logits, targets, old, adv)
+    # a few steps of the 64-bit logarithm, exponential and sums (1.2e-15 of the largest term), then one rounding to fp32
+    assert float(p.loss.detach()) == pytest.approx(float(want), abs=20 * 2**-52, rel=2**-24)
+    assert float(p.clipped) == 0
