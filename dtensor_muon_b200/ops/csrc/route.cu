@@ -57,30 +57,22 @@ struct Args {
   void* dlogits;
 };
 
-// Expert of a lane's j-th value: whole 8-value words lie next to each other across the lanes.
-template <int LPR>
-__device__ __forceinline__ int expert_of(int lane, int j) { return (j >> 3) * LPR * 8 + lane * 8 + (j & 7); }
+constexpr int kPerLane = 8;  // logits next to each other on each lane, where a row lies on one to eight lanes
 
-template <typename T, int LPR, int VPL>
-__device__ __forceinline__ void load_row(const Args& a, int row, bool in, int lane, float (&x)[VPL]) {
+template <typename T>
+__device__ __forceinline__ void load_row(const Args& a, int row, bool in, int lane, float (&x)[kPerLane]) {
   const T* p = static_cast<const T*>(a.logits) + (long long)row * a.stride;
+  const int e = lane * kPerLane;
 #pragma unroll
-  for (int j = 0; j < VPL; j += 8) {
-    const int e = expert_of<LPR>(lane, j);
-    float v[8];
+  for (int k = 0; k < kPerLane; ++k) x[k] = -INFINITY;
+  if (in) {
+    if (a.vec) {
+      if (e < a.experts) load8t<T>(p + e, x);
+    } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = -INFINITY;
-    if (in) {
-      if (a.vec) {
-        if (e < a.experts) load8t<T>(p + e, v);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (e + k < a.experts) v[k] = to_float(p[e + k]);
-      }
+      for (int k = 0; k < kPerLane; ++k)
+        if (e + k < a.experts) x[k] = to_float(p[e + k]);
     }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) x[j + k] = v[k];
   }
 }
 
@@ -128,9 +120,9 @@ __device__ __forceinline__ void write_part(const Args& a, const float* join_p, c
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0;
 }
 
-template <typename T, int LPR, int VPL>
+template <typename T, int LPR>
 __global__ void __launch_bounds__(kThreads) route_kernel(const Args a) {
-  constexpr int kGroups = kThreads / LPR, kExperts = LPR * VPL;
+  constexpr int VPL = kPerLane, kGroups = kThreads / LPR, kExperts = LPR * VPL;
   constexpr int kTop = kExperts < kMaxTopK ? kExperts : kMaxTopK;
   constexpr int kStash = 2 * kGroups * kTop, kJoin = 2 * kWarps * (kExperts + 1);
   __shared__ uint32_t smem[kStash > kJoin ? kStash : kJoin];
@@ -145,10 +137,10 @@ __global__ void __launch_bounds__(kThreads) route_kernel(const Args a) {
     const bool in = row < a.tokens;
     const bool valid = in && (!a.mask || a.mask[row]);
     float x[VPL];
-    load_row<T, LPR, VPL>(a, row, in, lane, x);
+    load_row<T>(a, row, in, lane, x);
     uint32_t key[VPL];
 #pragma unroll
-    for (int j = 0; j < VPL; ++j) key[j] = expert_of<LPR>(lane, j) < a.experts ? order_key(x[j]) : 0u;
+    for (int j = 0; j < VPL; ++j) key[j] = lane * VPL + j < a.experts ? order_key(x[j]) : 0u;
     uint32_t picked = 0;  // bit j: the lane's j-th expert is chosen
     float top = 0.f, total = 0.f;
     for (int i = 0; i < a.top_k; ++i) {
@@ -158,7 +150,7 @@ __global__ void __launch_bounds__(kThreads) route_kernel(const Args a) {
       for (int j = 0; j < VPL; ++j)
         if (key[j] > best) {  // within a lane, a later value has a higher index
           best = key[j];
-          at = expert_of<LPR>(lane, j);
+          at = lane * VPL + j;
         }
 #pragma unroll
       for (int o = LPR / 2; o > 0; o >>= 1) {
@@ -171,7 +163,7 @@ __global__ void __launch_bounds__(kThreads) route_kernel(const Args a) {
       }
 #pragma unroll
       for (int j = 0; j < VPL; ++j)
-        if (expert_of<LPR>(lane, j) == at) {
+        if (lane * VPL + j == at) {
           key[j] = 0;
           picked |= 1u << j;
         }
@@ -234,8 +226,8 @@ __global__ void __launch_bounds__(kThreads) route_kernel(const Args a) {
   if ((threadIdx.x & 31) < LPR) {
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
-      join_p[warp * (kExperts + 1) + expert_of<LPR>(lane, j)] = sum_p[j];
-      join_c[warp * (kExperts + 1) + expert_of<LPR>(lane, j)] = sum_c[j];
+      join_p[warp * (kExperts + 1) + lane * VPL + j] = sum_p[j];
+      join_c[warp * (kExperts + 1) + lane * VPL + j] = sum_c[j];
     }
     if (lane == 0) {
       join_p[warp * (kExperts + 1) + kExperts] = sum_z;
@@ -247,20 +239,24 @@ __global__ void __launch_bounds__(kThreads) route_kernel(const Args a) {
 
 // ------------------------------------------------------------------ a warp per row
 
+// A lane's values as they lie in memory, in words of 16 bytes, or of 8 for four 16-bit values.
+template <typename T, int VPL>
+union LaneWords {
+  using W = std::conditional_t<VPL * sizeof(T) == 8, uint2, uint4>;
+  static constexpr int kWords = VPL * sizeof(T) / sizeof(W);
+  W w[kWords];
+  T t[VPL];
+};
+
 // VPL logits next to each other on each lane: lane order is index order.
 template <typename T, int VPL>
 __device__ __forceinline__ void load_lane(const Args& a, int row, int lane, float (&x)[VPL]) {
   const T* p = static_cast<const T*>(a.logits) + (long long)row * a.stride + lane * VPL;
   if (a.vec) {  // whole: the row ends with a lane, and every lane's share is on its own boundary
-    constexpr int kBytes = VPL * sizeof(T) < 16 ? VPL * sizeof(T) : 16;
-    using W = std::conditional_t<kBytes == 16, uint4, std::conditional_t<kBytes == 8, uint2, uint32_t>>;
-    union {
-      W w[VPL * sizeof(T) / kBytes];
-      T t[VPL];
-    } u;
+    LaneWords<T, VPL> u;
     if (lane * VPL < a.experts) {
 #pragma unroll
-      for (int i = 0; i < (int)(VPL * sizeof(T) / kBytes); ++i) u.w[i] = __ldg(reinterpret_cast<const W*>(p) + i);
+      for (int i = 0; i < u.kWords; ++i) u.w[i] = __ldg(reinterpret_cast<const typename LaneWords<T, VPL>::W*>(p) + i);
     }
 #pragma unroll
     for (int j = 0; j < VPL; ++j) x[j] = lane * VPL < a.experts ? to_float(u.t[j]) : -INFINITY;
@@ -523,17 +519,12 @@ __global__ void __launch_bounds__(kThreads, VPL == 16 ? 2 : 4) route_warp_grad_k
       for (int j = 0; j < VPL; ++j) x[j] = 0.f;
     }
     if (a.vec_out) {
-      constexpr int kBytes = VPL * sizeof(T) < 16 ? VPL * sizeof(T) : 16;
-      using W = std::conditional_t<kBytes == 16, uint4, std::conditional_t<kBytes == 8, uint2, uint32_t>>;
-      union {
-        W w[VPL * sizeof(T) / kBytes];
-        T t[VPL];
-      } u;
+      LaneWords<T, VPL> u;
 #pragma unroll
       for (int j = 0; j < VPL; ++j) u.t[j] = from_float<T>(x[j]);
       if (lane * VPL < a.experts) {
 #pragma unroll
-        for (int i = 0; i < (int)(VPL * sizeof(T) / kBytes); ++i) reinterpret_cast<W*>(out)[i] = u.w[i];
+        for (int i = 0; i < u.kWords; ++i) reinterpret_cast<typename LaneWords<T, VPL>::W*>(out)[i] = u.w[i];
       }
     } else {
 #pragma unroll
@@ -543,9 +534,9 @@ __global__ void __launch_bounds__(kThreads, VPL == 16 ? 2 : 4) route_warp_grad_k
   }
 }
 
-template <typename T, int LPR, int VPL>
+template <typename T, int LPR>
 __global__ void __launch_bounds__(kThreads) route_grad_kernel(const Args a) {
-  constexpr int kGroups = kThreads / LPR, kExperts = LPR * VPL;
+  constexpr int VPL = kPerLane, kGroups = kThreads / LPR, kExperts = LPR * VPL;
   __shared__ float share[kExperts];  // c_e / (N k)
   __shared__ int choices;
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
@@ -558,7 +549,7 @@ __global__ void __launch_bounds__(kThreads) route_grad_kernel(const Args a) {
     const bool in = row < a.tokens;
     const bool valid = in && (!a.mask || a.mask[row]);
     float x[VPL];
-    load_row<T, LPR, VPL>(a, row, valid, lane, x);
+    load_row<T>(a, row, valid, lane, x);
     uint32_t picked = 0;
     float dg[VPL] = {};
     if (valid && a.dgates) {
@@ -568,7 +559,7 @@ __global__ void __launch_bounds__(kThreads) route_grad_kernel(const Args a) {
         const float d = to_float(static_cast<const T*>(a.dgates)[at]);
 #pragma unroll
         for (int j = 0; j < VPL; ++j)
-          if (expert_of<LPR>(lane, j) == expert) {
+          if (lane * VPL + j == expert) {
             dg[j] = d;
             picked |= 1u << j;
           }
@@ -585,7 +576,7 @@ __global__ void __launch_bounds__(kThreads) route_grad_kernel(const Args a) {
     for (int j = 0; j < VPL; ++j) {
       x[j] = ex2((x[j] - m) * kLog2e);
       s += x[j];
-      mix = fmaf(share[expert_of<LPR>(lane, j)], x[j], mix);
+      mix = fmaf(share[lane * VPL + j], x[j], mix);
       if ((picked >> j) & 1) {
         s_top += x[j];
         dot = fmaf(x[j], dg[j], dot);
@@ -600,23 +591,19 @@ __global__ void __launch_bounds__(kThreads) route_grad_kernel(const Args a) {
     dot *= inv_top;
     if (!in) continue;
     T* out = static_cast<T*>(a.dlogits) + (long long)row * a.experts;
+    const int e = lane * VPL;
 #pragma unroll
-    for (int j = 0; j < VPL; j += 8) {
-      const int e = expert_of<LPR>(lane, j);
-      float v[8];
+    for (int j = 0; j < VPL; ++j) {
+      float g = x[j] * inv * fmaf(by_balance, share[e + j], all);
+      if ((picked >> j) & 1) g = fmaf(x[j] * inv_top, dg[j] - dot, g);
+      x[j] = valid ? g : 0.f;
+    }
+    if (a.vec_out) {
+      if (e < a.experts) store8t<T>(out + e, x);
+    } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        float g = x[j + k] * inv * fmaf(by_balance, share[e + k], all);
-        if ((picked >> (j + k)) & 1) g = fmaf(x[j + k] * inv_top, dg[j + k] - dot, g);
-        v[k] = valid ? g : 0.f;
-      }
-      if (a.vec_out) {
-        if (e < a.experts) store8t<T>(out + e, v);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (e + k < a.experts) out[e + k] = from_float<T>(v[k]);
-      }
+      for (int j = 0; j < VPL; ++j)
+        if (e + j < a.experts) out[e + j] = from_float<T>(x[j]);
     }
   }
 }
@@ -632,10 +619,10 @@ void with_layout(const at::Tensor& logits, F&& f) {
   with_element(logits.scalar_type(), [&](auto* t) {
     const int e = (int)logits.size(1);
     using std::integral_constant;
-    if (e <= 8) f(t, integral_constant<int, 1>(), integral_constant<int, 8>());
-    else if (e <= 16) f(t, integral_constant<int, 2>(), integral_constant<int, 8>());
-    else if (e <= 32) f(t, integral_constant<int, 4>(), integral_constant<int, 8>());
-    else if (e <= 64) f(t, integral_constant<int, 8>(), integral_constant<int, 8>());
+    if (e <= 8) f(t, integral_constant<int, 1>(), integral_constant<int, kPerLane>());
+    else if (e <= 16) f(t, integral_constant<int, 2>(), integral_constant<int, kPerLane>());
+    else if (e <= 32) f(t, integral_constant<int, 4>(), integral_constant<int, kPerLane>());
+    else if (e <= 64) f(t, integral_constant<int, 8>(), integral_constant<int, kPerLane>());
     else if (e <= 128) f(t, integral_constant<int, 32>(), integral_constant<int, 4>());
     else if (e <= 256) f(t, integral_constant<int, 32>(), integral_constant<int, 8>());
     else f(t, integral_constant<int, 32>(), integral_constant<int, 16>());
@@ -643,7 +630,7 @@ void with_layout(const at::Tensor& logits, F&& f) {
 }
 
 // Values that a lane has next to each other.
-int per_lane(int experts) { return experts <= 64 ? 8 : experts <= 128 ? 4 : experts <= 256 ? 8 : 16; }
+int per_lane(int experts) { return experts <= 64 ? kPerLane : experts <= 128 ? 4 : experts <= 256 ? 8 : 16; }
 
 // Whether rows `stride` elements apart can be moved in a lane's whole words, of up to 16 bytes.
 bool whole_words(const void* p, int64_t rows, int64_t stride, int experts, int64_t size) {
@@ -707,7 +694,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> route_fwd
     a.sum_p = reinterpret_cast<float*>(a.ticket + 2);
     a.sum_c = reinterpret_cast<int*>(a.sum_p + (e + 1) * ctas);
     if constexpr (L == 32) route_warp_kernel<T, V><<<ctas, kThreads, 0, stream>>>(a);
-    else route_kernel<T, L, V><<<ctas, kThreads, 0, stream>>>(a);
+    else route_kernel<T, L><<<ctas, kThreads, 0, stream>>>(a);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
     const int joins = (int)((e + 1 + kJoinThreads / 32 - 1) / (kJoinThreads / 32));
     route_join_kernel<<<joins, kJoinThreads, 0, stream>>>(a, ctas, balance.template mutable_data_ptr<float>(),
@@ -757,7 +744,7 @@ at::Tensor route_bwd(const OptTensor& dgates, const OptTensor& dbalance, const O
     const int ctas = (int)std::min<int64_t>((a.tokens + groups - 1) / groups, (int64_t)sms * (L == 32 ? 4 : 8));
     const auto stream = at::cuda::getCurrentCUDAStream();
     if constexpr (L == 32) route_warp_grad_kernel<T, V><<<ctas, kThreads, 0, stream>>>(a);
-    else route_grad_kernel<T, L, V><<<ctas, kThreads, 0, stream>>>(a);
+    else route_grad_kernel<T, L><<<ctas, kThreads, 0, stream>>>(a);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   });
   count_launches(1);
