@@ -286,7 +286,11 @@ def route_composition(logits: Tensor, top_k: int, mask: Tensor | None) -> tuple[
     n = valid.sum().clamp(min=1).to(x.dtype)
     share = counts.to(x.dtype) / (n * top_k)
     balance = e * (share * (torch.softmax(x, dim=1) * valid[:, None]).sum(0) / n).sum()
-    z = (torch.logsumexp(x, dim=1).square() * valid).sum() / n
+    # not logsumexp, whose gradient is exp(x - lse): of large logits the rounded lse is off by more than the gradient may be
+    m = x.detach().amax(1, keepdim=True)
+    m = torch.where(m == -torch.inf, torch.zeros_like(m), m)
+    lse = m[:, 0] + torch.log(torch.exp(x - m).sum(1))
+    z = (lse * lse * valid).sum() / n
     wide = torch.float64 if logits.dtype == torch.float64 else torch.float32
     return gates.to(logits.dtype), experts, counts, balance.to(wide), z.to(wide)
 
