@@ -38,6 +38,8 @@ composition of the same math.
 
 from __future__ import annotations
 
+import importlib.util
+
 import torch
 import torch.nn.functional as F
 from torch import Tensor
@@ -468,6 +470,12 @@ def _zeropower_cpu(x: Tensor, steps: int, strategy: str, eps: float) -> Tensor:
 @zeropower.register_fake
 def _zeropower_fake(x, steps, strategy, eps):
     return x.new_empty(x.shape, dtype=torch.bfloat16)
+
+
+# The extension registers the CUDA kernels of the operators above when it is loaded: torch.ops.dmb has to find them whoever
+# calls it first (an exported program, say, which no longer goes through ops.model_ops).
+if importlib.util.find_spec("dtensor_muon_b200._C") is not None:
+    _ext.available()
 
 
 __all__ = ["cross_entropy", "cross_entropy_backward", "gram", "rope", "swiglu", "swiglu_backward", "zeropower"]
