@@ -16,21 +16,22 @@
 // row, from x_y - m and s: differences of log-probabilities nearly cancel, and rounding them first
 // would be what is lost. Rows that do not count are not read.
 //
-// Bound by memory, with the exponentials (16 a cycle and SM) close behind: arithmetic is packed,
-// two fp32 values to an instruction, and 16-bit logits are added to fp32 without unpacking. Measured on one B200, alone on the device (6.45 TB/s copied):
-//   scoring 4096 rows of 32000 bf16        46 us, 5.7 TB/s (262 MB)
+// Bound by memory, with the exponentials (16 a cycle and SM) close behind: arithmetic is packed, two fp32 values to an
+// instruction, and 16-bit logits are added to fp32 without unpacking. Measured on one B200 (6.45 TB/s copied), between
+// events around queued calls, the launches' gaps and the small kernels among them:
+//   scoring 4096 rows of 32000 bf16        48 us, 5.5 TB/s (262 MB); fp32 78 us, 6.7 TB/s
 //   policy loss and gradient, 4096 rows of 128256 bf16, a quarter masked
-//                                         355 us, 5.2 TB/s (1.84 GB; two passes took 448)
+//                                         364 us, 5.1 TB/s (1.84 GB; in two passes 418); 677 for a loss gradient that is not
+//                                         1, for which the gradient is computed again
 //   preference loss and gradient, 4096 rows of 32000 bf16, 40 % masked
-//                                         106 us, 5.4 TB/s (577 MB: the logits are read twice, as
-//                                         a coefficient hangs on the sums of both sequences)
+//                                         113 us, 5.1 TB/s (577 MB: the logits are read twice, as a coefficient hangs on the
+//                                         sums of both sequences); fp32 218 us
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <cooperative_groups.h>
-
 
 #include "train_ops.h"
 #include "vec.cuh"
@@ -361,14 +362,15 @@ __global__ void __launch_bounds__(32 * kWarpRows) warp_row_kernel(const RowArgs 
 
 constexpr int kRowThreads = 256;
 // With GRAD a row is split until a part is no longer than this: fewer rows at once, which are still in the L2 when the
-// gradient is written. 4096 rows of 128256 bf16 logits, a quarter of them masked, took 380 us in four parts, 395 in two, 406
-// in one (each row then comes from memory twice), and 421 in eight, which have too little to do between two barriers.
+// gradient is written. 4096 rows of 128256 bf16 logits, a quarter of them masked, take 364 us in four parts, 443 in two, 480
+// in one (each row then comes from memory twice), and 420 in eight, which have too little to do between two barriers.
 constexpr int kGradPart = 80 * 1024;
 
 // A cluster of CTAs per row, most often of one: with fewer rows than the GPU has room for a row is split, and the parts are
 // joined through the first CTA's shared memory. With GRAD the row's gradient follows at once, while the row is in the L2.
 // Registers for six CTAs to an SM, five for fp32, which the compiler does not come to by itself. With GRAD the rows above
-// take 350 us so, 380 with four and 397 with eight (which spill); 4096 rows of 32000 take 47 us without GRAD, 54 with four.
+// take 364 us so, 382 with four and 435 with eight (which spill); 4096 rows of 32000 take 48 us without GRAD, 49 with four and
+// 51 with eight.
 template <typename T, Mode MODE, bool GRAD>
 __global__ void __launch_bounds__(kRowThreads, sizeof(T) == 2 ? 6 : 5) row_kernel(const RowArgs a) {
   constexpr int NT = kRowThreads;
@@ -389,7 +391,7 @@ __global__ void __launch_bounds__(kRowThreads, sizeof(T) == 2 ? 6 : 5) row_kerne
   const T* p = row_of<T>(a.logits, a.stride_b, a.stride_s, a.seq, row);
   const int head = head_of(p, a.vocab), vecs = (a.vocab - head) / 8;
   const int each = (vecs + split - 1) / split, v0 = min(rank * each, vecs), v1 = min(v0 + each, vecs);
-  if (GRAD && tid == 0 && v1 > v0)  // the whole part to the L2, at once: 381 to 364 us. (Without GRAD 48 become 51.)
+  if (GRAD && tid == 0 && v1 > v0)  // the whole part to the L2, at once: 383 to 364 us. (Without GRAD 48 become 49.)
     asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p + head + (long long)v0 * 8),
                  "r"((uint32_t)(v1 - v0) * 8 * (uint32_t)sizeof(T))
                  : "memory");
@@ -601,8 +603,8 @@ void check_values(const at::Tensor& v, const at::Tensor& targets, const char* na
 }
 
 // Whether rows go to a warp each: where they are short and many. Warp and CTA, log-probabilities and gradients of bf16 rows:
-// 4096 of 1024 4.1 + 4.3 and 13 + 13 us, 16384 of 4096 33 + 40 and 62 + 63 us, 4096 of 8192 19 + 19 and 20 + 21 us; 74 of
-// 1024 2.6 + 2.9 and 2.8 + 2.4 us, 74 of 4096 3.9 + 5.2 and 2.9 + 2.5 us.
+// 4096 of 1024 6 + 6 and 14 + 14 us, 16384 of 4096 29 + 47 and 63 + 66 us, 4096 of 8192 17 + 23 and 21 + 27 us, 1184 of 8192
+// 8 + 10 and 8 + 8 us; 600 of 4096 6 + 6 us either way, 74 of 4096 6 + 6 and 4 + 4 us.
 bool in_warps(const Rows& r) {
   return r.vocab <= 8192 && r.rows >= 8 * at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
 }
@@ -644,7 +646,7 @@ void launch_rows(const Rows& r, RowArgs& a, cudaStream_t stream) {
       return;
     }
     // Few rows: split each until every SM has two CTAs or a part is down to two rounds of its CTA's loads. (Rows of 128256
-    // bf16, split and whole: 4 of them 4.8 and 10 us, 64 7.1 and 13 us, 150 15 and 20 us.)
+    // bf16, split and whole: 4 of them 6 and 12 us, 64 8 and 12 us, 150 16 and 21 us.)
     const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
     int split = 1;
     while (split < 8 && (int64_t)r.rows * split < 2 * sms && r.vocab / split > 2 * kRowThreads * 8 * kUnroll) split *= 2;

@@ -12,9 +12,10 @@
 // Queries and keys share one launch. All of it is computed in fp32 and rounded once. Unpacked
 // arithmetic would take longer than the memory: the first and the second values of a lane's four
 // rotated pairs lie in packed registers, two and two, so that nothing is shuffled between them.
-// Measured on one B200: 4096 tokens of 32 + 8 heads of 128 bf16 take 18 us forward (84 MB, 4.7 TB/s)
-// and 25 us backward (126 MB, 5.0 TB/s; 39 us before the arithmetic was packed, 31 before the loads
-// ran ahead of it), and 3 us for the sum of the weights' gradients over the CTAs.
+// Measured on one B200, between events around queued calls: 4096 tokens of 32 + 8 heads of 128 bf16 take 18.5 us
+// forward (84 MB, 4.5 TB/s) and 31 us backward (126 MB, 4.0 TB/s) with the 3 us for the sum of the weights' gradients
+// over the CTAs; 16384 tokens 64 and 92 us (5.2 and 5.5 TB/s); 4096 tokens of fp32 32 and 66 us. An RMS norm and a
+// rotation one after the other, each with its gradient, take 443 us for the 51 of the 4096 tokens here.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
@@ -414,8 +415,8 @@ Args args_of(Kept& t, const at::Tensor& q, const at::Tensor& k, const at::Tensor
 }
 
 // Heads per group: four share a token's angles (two in the backward pass) once they still fill half the GPU's lanes. 40
-// heads of 128 bf16, forward and backward with one head and with four (two): 8 tokens 2.0 + 3.7 and 2.3 + 3.8 us, 512
-// tokens 4.3 + 6.5 and 3.5 + 6.1 us, 4096 tokens 26 + 42 and 18 + 31 us (before the backward's loads ran ahead).
+// heads of 128 bf16, forward and backward with one head and with four (two): 8 tokens 4.2 + 9.4 and 4.2 + 10.3 us, 512
+// tokens 6.2 + 12.4 and 5.3 + 12.4 us, 1024 8.3 + 16.5 and 6.2 + 14.4 us, 4096 tokens 26 + 37 and 18.5 + 31 us.
 int heads_per_group(const at::Tensor& q, const at::Tensor& k) {
   const int64_t rows = q.size(0) * q.size(1) * (q.size(2) + k.size(2));
   const int64_t lanes = (int64_t)at::cuda::getCurrentDeviceProperties()->multiProcessorCount * 512;

@@ -9,9 +9,13 @@
 // Up to 64 experts a row lies on one to eight lanes, eight logits on each; above, on a warp, four to 16 logits on each
 // lane. The choice takes k rounds of a maximum over the row by (value, index); on a warp the lanes sort their logits first,
 // and a round is one redux over order-preserving integer keys and a ballot. Every group of lanes
-// walks over rows and keeps its sums of p and its counts in registers; a CTA joins them in a fixed order and writes one
-// part, and a second kernel sums the parts in 64 bits. So nothing that is rounded is summed by atomics, and a run gives
-// the same bits each time. What bounds it: launches for small batches, the instructions of the k rounds for many experts.
+// walks over rows and keeps its sums of p and of lse^2 in 32 bits and its counts in registers; a CTA joins them in a fixed
+// order, in 32 bits too, and writes one part, and a second kernel sums the parts in 64 bits. The longest chain of 32-bit
+// additions is a group's own rows, one in 592 CTAs times the groups of a CTA (4 of 65536 rows of 64 experts, 14 of 65536 rows
+// of 128), then at most five over its warp and eight over the warps. Nothing that is rounded is summed by atomics, and a run
+// gives the same bits each time. What bounds it: launches for small batches (16384 rows of 8, top 2: 16 us for three kernels),
+// the instructions of the k rounds and latency for many experts (65536 bf16 rows, top 8, forward + backward: 8 experts 17 + 7
+// us, 64 39 + 21 us, 128 47 + 25 us, 256 73 + 43 us, where the bytes alone take 1 to 12 us).
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
@@ -612,8 +616,8 @@ __global__ void __launch_bounds__(kThreads) route_grad_kernel(const Args a) {
 
 // f(T, LPR, VPL): up to 64 experts as few lanes per row as hold it at eight logits each, so that a warp has four rows or
 // more at once; above a warp per row, whose rounds are cheaper and whose other work is dearer. 65536 bf16 rows forward +
-// backward, on lanes and on a warp: 64 experts 14 + 12 and 21 + 21 us at top 2, 28 + 19 and 29 + 20 us at top 8; 128
-// experts 27 + 21 and 28 + 24 us at top 2, 56 + 33 and 37 + 24 us at top 8.
+// backward, on lanes and on a warp: 64 experts 24 + 14 and 37 + 25 us at top 2, 39 + 21 and 47 + 25 us at top 8; 128
+// experts 37 + 23 and 37 + 25 us at top 2, 66 + 35 and 47 + 25 us at top 8.
 template <typename F>
 void with_layout(const at::Tensor& logits, F&& f) {
   with_element(logits.scalar_type(), [&](auto* t) {
