@@ -244,6 +244,20 @@ def test_a_step_is_captured_after_an_eager_one():
     _near({n: p.grad.float() for n, p in model.named_parameters()}, {n: g.float() for n, g in want.items()}, 2**-8)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("step", ["policy_step", "preference_step"])
+def test_a_compiled_model_gpu(step):
+    model = _built(_config(), "cuda")
+    tokens, targets, mask, _ = _batch("cuda")
+    want = _router_gradients(model, tokens)
+    seen = _seen(model)
+    trainer = Trainer(torch.compile(model, backend="aot_eager"), torch.optim.SGD(model.parameters(), lr=0.0))
+    for _ in range(2):
+        _take(trainer, step, tokens, targets, mask)
+        # fp32; sums over tokens may come in another order
+        _near({n: seen[n] for n in want}, want, 1e-5)
+
+
 def test_other_callables_are_trained_as_they_are():
     """A function has no layers to look through, and a foreign model's own ``aux_loss`` is not ours to call."""
     model = nn.Sequential(nn.Embedding(512, 8), nn.Linear(8, 512))
