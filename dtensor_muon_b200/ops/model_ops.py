@@ -13,6 +13,9 @@ be seen from the host without waiting for the device: the CPU raises, and a
 kernel makes its results NaN and records an error that
 ``ops._ext.check_device_errors`` raises. Gradients of gradients are refused.
 
+``torch.func``: ``vmap``, ``grad`` and ``jvp`` go through the composition; of a
+kernel ``vmap`` takes the forward, sample by sample, and its gradient raises.
+
 CUDA graphs: both directions can be captured. As for any autograd call,
 capture a backward pass only while no eager graph of the same leaves lives.
 """
